@@ -39,6 +39,8 @@ EXPORTED = (
     "esa_init_device", "esa_build_dense_mask",
     "esa_elastic_fwd_naive", "esa_gather_bwd_workspace_size", "esa_sparse_bwd",
     "esa_elastic_bwd_rows", "esa_reachability",
+    "esa_qk_norm_rope_fwd", "esa_qk_norm_rope_append", "esa_qk_norm_rope_bwd_workspace_size",
+    "esa_qk_norm_rope_bwd",
 )
 
 
@@ -102,6 +104,32 @@ class EsaNaiveOpts(ctypes.Structure):
         ("weights", ctypes.c_void_p),
         ("weights_stride_b", ctypes.c_int64), ("weights_stride_h", ctypes.c_int64),
         ("weights_stride_s", ctypes.c_int64),
+    ]
+
+
+class EsaRotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("num_heads", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("seq_len", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("rotary_dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("kv_len", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("inv_freq", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("position_stride_b", ctypes.c_int64),
+    ] + [f for name in ("q", "k", "v", "q_out", "k_out", "v_out", "q_grad", "k_grad")
+         for f in ((name, ctypes.c_void_p), (f"{name}_stride_b", ctypes.c_int64),
+                   (f"{name}_stride_h", ctypes.c_int64), (f"{name}_stride_s", ctypes.c_int64))] + [
+        ("q_weight_grad", ctypes.c_void_p),
+        ("k_weight_grad", ctypes.c_void_p),
     ]
 
 
@@ -186,6 +214,14 @@ def load() -> ctypes.CDLL:
     i32 = ctypes.c_int32
     lib.esa_reachability.restype = st
     lib.esa_reachability.argtypes = [i32, i32, i32, i32, i32, vp, vp, vp, vp]
+    lib.esa_qk_norm_rope_fwd.restype = st
+    lib.esa_qk_norm_rope_fwd.argtypes = [P(EsaRotaryArgs), vp]
+    lib.esa_qk_norm_rope_append.restype = st
+    lib.esa_qk_norm_rope_append.argtypes = [P(EsaRotaryArgs), vp]
+    lib.esa_qk_norm_rope_bwd_workspace_size.restype = st
+    lib.esa_qk_norm_rope_bwd_workspace_size.argtypes = [P(EsaRotaryArgs), P(ctypes.c_size_t)]
+    lib.esa_qk_norm_rope_bwd.restype = st
+    lib.esa_qk_norm_rope_bwd.argtypes = [P(EsaRotaryArgs), vp, ctypes.c_size_t, vp]
     _lib = lib
     return lib
 

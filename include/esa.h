@@ -507,6 +507,73 @@ esa_status esa_reachability(int32_t seq_len, int32_t attention_length,
                             int32_t position, uint32_t* reach, uint32_t* work,
                             int32_t* layer_counts, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Norm and rotation of queries and keys, head by head (no reference
+ * counterpart: the reference's layer takes q and k as its caller prepared
+ * them).
+ *
+ *   n = x / sqrt(mean(x^2) + eps),  y = R(p) (n * gain)
+ *
+ * over each head's head_dim elements; R(p) turns pair i of the first
+ * rotary_dim elements by p * inv_freq[i]: elements (i, i + rotary_dim / 2),
+ * or (2 i, 2 i + 1) when interleaved.  Angles are float64, everything else
+ * float32, rounded once.  head_dim is a multiple of 4 up to 256, rotary_dim
+ * one of 8 from 8 to head_dim.  Rows are read and written 16 bytes at a time
+ * (8 where a 16-bit head_dim is no multiple of 8, or where the halves of a
+ * 16-bit rotary_dim are none): pointers and strides have to be so aligned.
+ */
+typedef struct esa_rotary_args {
+  esa_dtype dtype;        /* q, k, v, their outputs and gradients */
+  esa_dtype weight_dtype; /* the gains and their gradients */
+  int32_t batch, num_heads, num_kv_heads, seq_len, head_dim, rotary_dim;
+  int32_t interleaved;    /* 0 or 1 */
+  int32_t kv_len;         /* append: rows of the caches */
+  float eps;              /* >= 0 */
+  const void* q_weight;   /* gains [head_dim], or NULL (1) */
+  const void* k_weight;
+  const double* inv_freq; /* device, [rotary_dim / 2]: radians per position */
+  const int64_t* positions;   /* device, [seq_len] rows per sequence */
+  int64_t position_stride_b;  /* 0: shared by the batch */
+  const void* q;          /* [batch, num_heads, seq_len, head_dim] */
+  int64_t q_stride_b, q_stride_h, q_stride_s;
+  const void* k;          /* [batch, num_kv_heads, seq_len, head_dim] */
+  int64_t k_stride_b, k_stride_h, k_stride_s;
+  const void* v;          /* append: the new value rows, as k */
+  int64_t v_stride_b, v_stride_h, v_stride_s;
+  void* q_out;            /* rotated q; backward: dq */
+  int64_t q_out_stride_b, q_out_stride_h, q_out_stride_s;
+  void* k_out;            /* rotated k; append: the key cache; backward: dk */
+  int64_t k_out_stride_b, k_out_stride_h, k_out_stride_s;
+  void* v_out;            /* append: the value cache */
+  int64_t v_out_stride_b, v_out_stride_h, v_out_stride_s;
+  const void* q_grad;     /* backward: gradients of q_out and k_out */
+  int64_t q_grad_stride_b, q_grad_stride_h, q_grad_stride_s;
+  const void* k_grad;
+  int64_t k_grad_stride_b, k_grad_stride_h, k_grad_stride_s;
+  void* q_weight_grad;    /* backward: [head_dim], or NULL */
+  void* k_weight_grad;
+} esa_rotary_args;
+
+/* q_out, k_out = norm and rotation of q, k at `positions` (any int64). */
+esa_status esa_qk_norm_rope_fwd(const esa_rotary_args* a, void* stream);
+
+/* The same for new rows of sequences that keep caches [batch, num_kv_heads,
+ * kv_len, head_dim]: q_out gets the queries, k_out and v_out (the caches) the
+ * keys and values at the rows' positions.  Row s of a sequence belongs at its
+ * first position (a negative one counting from kv_len) + s; a row whose
+ * position is another one or lies outside the cache writes no cache row and
+ * gets a NaN query.  Nothing else of the caches is written. */
+esa_status esa_qk_norm_rope_append(const esa_rotary_args* a, void* stream);
+
+/* Host only.  Workspace of esa_qk_norm_rope_bwd (0 without gain gradients). */
+esa_status esa_qk_norm_rope_bwd_workspace_size(const esa_rotary_args* a, size_t* bytes);
+
+/* Gradients: q_out, k_out = dq, dk from q, k, q_grad and k_grad, and the
+ * gains' gradients where their pointers are given (sums in a fixed order, no
+ * atomics).  The workspace is 16-byte aligned. */
+esa_status esa_qk_norm_rope_bwd(const esa_rotary_args* a, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
