@@ -27,7 +27,7 @@ BUILD = os.path.join(HERE, "_build")
 SOURCES = ["esa_capi.hip", "esa_layout.hip", "esa_fwd_tile.hip", "esa_fwd_band.hip",
            "esa_bwd_band.hip", "esa_fwd_gather.hip", "esa_bwd_gather.hip", "esa_bwd.hip",
            "esa_reach.hip", "esa_bwd_fix.hip", "esa_fwd_window.hip", "esa_capi_layer.hip",
-           "esa_rotary.hip"]
+           "esa_rotary.hip", "esa_sink_fwd.hip", "esa_sink_bwd.hip", "esa_sink_decode.hip"]
 PROBE_SOURCES = ["esa_probe.hip"]
 LIB = os.path.join(HERE, "libesa.so")
 PROBE_LIB = os.path.join(HERE, "libesa_probe.so")

@@ -5,6 +5,7 @@
 
 #include "esa.h"
 #include "esa_rotary.hpp"
+#include "esa_sink.hpp"
 
 using namespace esa;
 
@@ -140,6 +141,156 @@ esa_status rotary_run(const esa_rotary_args* a, int mode, void* workspace, size_
   return launch_rotary(g, mode, (hipStream_t)stream) == hipSuccess ? ESA_OK : ESA_ERR_HIP;
 }
 
+constexpr int64_t kMaxKeys = int64_t(1) << 26;      // positions and rows are int32
+constexpr int64_t kMaxGrid = int64_t(1) << 24;      // workgroups of 256 work-items
+
+// 16-byte rows: base and strides
+esa_status sink_rows_ok(const void* p, int64_t sb, int64_t sh, int64_t ss, int elems) {
+  if (!aligned(p, 16) || sb % elems || sh % elems || ss % elems) return ESA_ERR_ALIGN;
+  return ESA_OK;
+}
+
+// a stage's rows lie within 2 GiB of its first one
+bool stage_span_ok(int64_t stride, int es) {
+  return stride >= 0 && stride < (int64_t(1) << 31) / (128 * es);
+}
+
+// The checks that the forward and the backward share.
+esa_status sink_check(esa_dtype dtype, int32_t batch, int32_t heads, int32_t kv_heads,
+                      int32_t q_len, int32_t kv_len, int32_t head_dim, float sm_scale,
+                      const esa_window* w) {
+  if (!w) return ESA_ERR_NULL;
+  if (!dtype_ok(dtype)) return ESA_ERR_DTYPE;
+  if (batch < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || q_len < 0 ||
+      kv_len < 1 || head_dim < 1 || w->window < 1 || w->sinks < 0 || w->position_stride_b < 0)
+    return ESA_ERR_SHAPE;
+  if (q_len > kMaxKeys || kv_len > kMaxKeys || (!w->positions && q_len > kv_len))
+    return ESA_ERR_SHAPE;
+  const int epc = dtype == ESA_F32 ? 4 : 8;
+  if (head_dim > 128 || head_dim % epc != 0) return ESA_ERR_UNSUPPORTED;
+  if (!(sm_scale > 0.f) || !std::isfinite(sm_scale)) return ESA_ERR_UNSUPPORTED;
+  if ((int64_t)batch * heads * ((q_len + 127) / 128) >= kMaxGrid ||
+      (int64_t)batch * kv_heads * ((kv_len + 127) / 128) >= kMaxGrid)
+    return ESA_ERR_SHAPE;
+  return ESA_OK;
+}
+
+void sink_pattern(SinkArgs& g, const esa_window* w) {
+  g.window = std::min(w->window, g.kv_len);
+  // (a window over the whole cache hides nothing that sinks could show)
+  g.sinks = g.window >= g.kv_len ? 0 : std::min(w->sinks, g.kv_len);
+  g.pos = w->positions;
+  g.pos_sb = w->position_stride_b;
+  g.first = w->first_key;
+  g.nqb = (g.q_len + 127) / 128;
+}
+
+// Few rows against many keys: the decode kernel (row tiles of 16 over the
+// heads that share a kv head, keys cut into ranges).
+bool sink_decodes(const SinkArgs& g) {
+  return (int64_t)g.groups * g.q_len <= 64 && (int64_t)g.B * g.H * g.q_len < kMaxGrid / 4;
+}
+
+void sink_splits(SinkArgs& g) {
+  g.row_tiles = (g.groups * g.q_len + 15) / 16;
+  const int64_t keys = std::min<int64_t>(g.kv_len, (int64_t)g.window + g.sinks + g.q_len);
+  const int64_t units = (int64_t)g.B * g.Hkv * g.row_tiles;
+  g.splits = (int)std::min<int64_t>((keys + 127) / 128, std::max<int64_t>(1, 1024 / units));
+}
+
+SinkArgs sink_fwd_args(const esa_fwd_args* a, const esa_window* w) {
+  SinkArgs g{};
+  g.q = a->q; g.k = a->k; g.v = a->v; g.o = a->o; g.lse = a->lse;
+  g.qsb = a->q_stride_b; g.qsh = a->q_stride_h; g.qss = a->q_stride_s;
+  g.ksb = a->k_stride_b; g.ksh = a->k_stride_h; g.kss = a->k_stride_s;
+  g.vsb = a->v_stride_b; g.vsh = a->v_stride_h; g.vss = a->v_stride_s;
+  g.osb = a->o_stride_b; g.osh = a->o_stride_h; g.oss = a->o_stride_s;
+  g.lsb = a->lse_stride_b; g.lsh = a->lse_stride_h;
+  g.B = a->batch; g.H = a->num_heads; g.Hkv = a->num_kv_heads; g.groups = g.H / g.Hkv;
+  g.q_len = a->q_len; g.kv_len = a->kv_len; g.d_real = a->head_dim;
+  g.elem = a->dtype;
+  g.sm_scale = a->sm_scale;
+  g.scale_log2 = (float)((double)a->sm_scale * 1.4426950408889634);
+  sink_pattern(g, w);
+  if (sink_decodes(g)) sink_splits(g);
+  return g;
+}
+
+// bytes of the decode kernel's parts: O [.., 16][D], then (m, l, n) [.., 16]
+size_t sink_fwd_workspace(const SinkArgs& g) {
+  if (!sink_decodes(g) || g.splits <= 1) return 0;
+  const size_t rows = (size_t)g.B * g.Hkv * g.row_tiles * g.splits * 16;
+  return rows * ((g.d_real <= 64 ? 64 : 128) + 3) * sizeof(float);
+}
+
+esa_status sink_fwd_shape(const esa_fwd_args* a, const esa_window* w) {
+  if (!a) return ESA_ERR_NULL;
+  return sink_check(a->dtype, a->batch, a->num_heads, a->num_kv_heads, a->q_len, a->kv_len,
+                    a->head_dim, a->sm_scale, w);
+}
+
+// Row stride of delta and lse2 (whole 16 bytes a head)
+int sink_qpad(int q_len) { return (q_len + 3) / 4 * 4; }
+
+// How the rows of a key block are cut.  A block is walked by one workgroup
+// while the grid fills the chip; a sinks' block, which every later row sees, is
+// cut into pieces of about a window block's rows.
+void sink_bwd_plan(SinkArgs& g) {
+  g.nkb = (g.kv_len + 127) / 128;
+  g.n_sink_blocks = std::min(g.nkb, (g.sinks + 127) / 128);
+  g.qpad = sink_qpad(g.q_len);
+  const int64_t blocks = (int64_t)g.B * g.Hkv * g.nkb;
+  const int64_t rows = std::min<int64_t>(g.q_len, (int64_t)g.window + 127);  // a block's, at most
+  const int64_t stages = (rows + 63) / 64 * g.groups;
+  g.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(stages / 4, 512 / blocks));
+  const int64_t ratio = ((int64_t)g.q_len + rows - 1) / rows;
+  const int64_t sink_blocks = std::max<int64_t>(1, (int64_t)g.B * g.Hkv * g.n_sink_blocks);
+  g.sink_chunks = (int)std::min<int64_t>(std::min<int64_t>(64, ratio * g.chunks),
+                                         std::max<int64_t>(1, 2048 / sink_blocks));
+}
+
+struct SinkBwdSizes {
+  size_t stat, part;  // bytes of delta (and of lse2), of the parts
+  size_t total() const { return 2 * stat + part; }
+};
+SinkBwdSizes sink_bwd_sizes(const SinkArgs& g) {
+  SinkBwdSizes z;
+  z.stat = ((size_t)g.B * g.H * g.qpad * sizeof(float) + 255) / 256 * 256;
+  const size_t cut = (g.sink_chunks > 1 || g.chunks > 1 ? (size_t)g.n_sink_blocks * g.sink_chunks : 0) +
+                     (g.chunks > 1 ? (size_t)(g.nkb - g.n_sink_blocks) * g.chunks : 0);
+  z.part = (size_t)g.B * g.Hkv * cut * 2 * 128 * (g.d_real <= 64 ? 64 : 128) * sizeof(float);
+  return z;
+}
+
+esa_status sink_bwd_shape(const esa_bwd_args* a, const esa_window* w) {
+  if (!a) return ESA_ERR_NULL;
+  return sink_check(a->dtype, a->batch, a->num_heads, a->num_kv_heads, a->q_len, a->kv_len,
+                    a->head_dim, a->sm_scale, w);
+}
+
+SinkArgs sink_bwd_args(const esa_bwd_args* a, const esa_window* w) {
+  SinkArgs g{};
+  g.q = a->q; g.k = a->k; g.v = a->v; g.o = (void*)a->o; g.dout = a->dout;
+  g.dq = a->dq; g.dk = a->dk; g.dv = a->dv; g.lse = (float*)a->lse;
+  g.qsb = a->q_stride_b; g.qsh = a->q_stride_h; g.qss = a->q_stride_s;
+  g.ksb = a->k_stride_b; g.ksh = a->k_stride_h; g.kss = a->k_stride_s;
+  g.vsb = a->v_stride_b; g.vsh = a->v_stride_h; g.vss = a->v_stride_s;
+  g.osb = a->o_stride_b; g.osh = a->o_stride_h; g.oss = a->o_stride_s;
+  g.dosb = a->dout_stride_b; g.dosh = a->dout_stride_h; g.doss = a->dout_stride_s;
+  g.dqsb = a->dq_stride_b; g.dqsh = a->dq_stride_h; g.dqss = a->dq_stride_s;
+  g.dksb = a->dk_stride_b; g.dksh = a->dk_stride_h; g.dkss = a->dk_stride_s;
+  g.dvsb = a->dv_stride_b; g.dvsh = a->dv_stride_h; g.dvss = a->dv_stride_s;
+  g.lsb = a->lse_stride_b; g.lsh = a->lse_stride_h;
+  g.B = a->batch; g.H = a->num_heads; g.Hkv = a->num_kv_heads; g.groups = g.H / g.Hkv;
+  g.q_len = a->q_len; g.kv_len = a->kv_len; g.d_real = a->head_dim;
+  g.elem = a->dtype;
+  g.sm_scale = a->sm_scale;
+  g.scale_log2 = (float)((double)a->sm_scale * 1.4426950408889634);
+  sink_pattern(g, w);
+  sink_bwd_plan(g);
+  return g;
+}
+
 }  // namespace
 
 extern "C" {
@@ -166,6 +317,84 @@ esa_status esa_qk_norm_rope_bwd_workspace_size(const esa_rotary_args* a, size_t*
 esa_status esa_qk_norm_rope_bwd(const esa_rotary_args* a, void* workspace, size_t workspace_bytes,
                                 void* stream) {
   return rotary_run(a, kRotBwd, workspace, workspace_bytes, stream);
+}
+
+esa_status esa_sink_window_fwd_workspace_size(const esa_fwd_args* a, const esa_window* w,
+                                              size_t* bytes) {
+  if (!bytes) return ESA_ERR_NULL;
+  const esa_status s = sink_fwd_shape(a, w);
+  if (s != ESA_OK) return s;
+  *bytes = a->batch == 0 || a->q_len == 0 ? 0 : sink_fwd_workspace(sink_fwd_args(a, w));
+  return ESA_OK;
+}
+
+esa_status esa_sink_window_fwd(const esa_fwd_args* a, const esa_window* w, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  esa_status s = sink_fwd_shape(a, w);
+  if (s != ESA_OK) return s;
+  if (a->batch == 0 || a->q_len == 0) return ESA_OK;
+  if (!a->q || !a->k || !a->v || !a->o) return ESA_ERR_NULL;
+  const int es = a->dtype == ESA_F32 ? 4 : 2, epc = 16 / es;
+  if (!stage_span_ok(a->k_stride_s, es) || !stage_span_ok(a->v_stride_s, es))
+    return ESA_ERR_UNSUPPORTED;
+  if ((s = sink_rows_ok(a->q, a->q_stride_b, a->q_stride_h, a->q_stride_s, epc)) != ESA_OK ||
+      (s = sink_rows_ok(a->k, a->k_stride_b, a->k_stride_h, a->k_stride_s, epc)) != ESA_OK ||
+      (s = sink_rows_ok(a->v, a->v_stride_b, a->v_stride_h, a->v_stride_s, epc)) != ESA_OK ||
+      (s = sink_rows_ok(a->o, a->o_stride_b, a->o_stride_h, a->o_stride_s, epc)) != ESA_OK)
+    return s;
+  SinkArgs g = sink_fwd_args(a, w);
+  const size_t need = sink_fwd_workspace(g);
+  if (need > 0) {
+    if (!workspace) return ESA_ERR_NULL;
+    if (!aligned(workspace, 16)) return ESA_ERR_ALIGN;
+    if (workspace_bytes < need) return ESA_ERR_CAPACITY;
+    g.partial = (float*)workspace;
+    g.part_ml = g.partial + (size_t)g.B * g.Hkv * g.row_tiles * g.splits * 16 *
+                                (g.d_real <= 64 ? 64 : 128);
+  }
+  const hipError_t e = sink_decodes(g) ? launch_sink_decode(g, (hipStream_t)stream)
+                                       : launch_sink_fwd(g, (hipStream_t)stream);
+  return e == hipSuccess ? ESA_OK : ESA_ERR_HIP;
+}
+
+esa_status esa_sink_window_bwd_workspace_size(const esa_bwd_args* a, const esa_window* w,
+                                              size_t* bytes) {
+  if (!bytes) return ESA_ERR_NULL;
+  const esa_status s = sink_bwd_shape(a, w);
+  if (s != ESA_OK) return s;
+  *bytes = a->batch == 0 || a->q_len == 0 ? 0 : sink_bwd_sizes(sink_bwd_args(a, w)).total();
+  return ESA_OK;
+}
+
+esa_status esa_sink_window_bwd(const esa_bwd_args* a, const esa_window* w, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  esa_status s = sink_bwd_shape(a, w);
+  if (s != ESA_OK) return s;
+  if (a->batch == 0 || a->q_len == 0) return ESA_OK;
+  if (!a->q || !a->k || !a->v || !a->o || !a->dout || !a->dq || !a->dk || !a->dv || !a->lse)
+    return ESA_ERR_NULL;
+  const int es = a->dtype == ESA_F32 ? 4 : 2, epc = 16 / es;
+  if (!stage_span_ok(a->k_stride_s, es) || !stage_span_ok(a->v_stride_s, es) ||
+      !stage_span_ok(a->q_stride_s, es) || !stage_span_ok(a->dout_stride_s, es))
+    return ESA_ERR_UNSUPPORTED;
+  if ((s = sink_rows_ok(a->q, a->q_stride_b, a->q_stride_h, a->q_stride_s, epc)) != ESA_OK ||
+      (s = sink_rows_ok(a->k, a->k_stride_b, a->k_stride_h, a->k_stride_s, epc)) != ESA_OK ||
+      (s = sink_rows_ok(a->v, a->v_stride_b, a->v_stride_h, a->v_stride_s, epc)) != ESA_OK ||
+      (s = sink_rows_ok(a->o, a->o_stride_b, a->o_stride_h, a->o_stride_s, epc)) != ESA_OK ||
+      (s = sink_rows_ok(a->dout, a->dout_stride_b, a->dout_stride_h, a->dout_stride_s, epc)) != ESA_OK ||
+      (s = sink_rows_ok(a->dq, a->dq_stride_b, a->dq_stride_h, a->dq_stride_s, epc)) != ESA_OK ||
+      (s = sink_rows_ok(a->dk, a->dk_stride_b, a->dk_stride_h, a->dk_stride_s, epc)) != ESA_OK ||
+      (s = sink_rows_ok(a->dv, a->dv_stride_b, a->dv_stride_h, a->dv_stride_s, epc)) != ESA_OK)
+    return s;
+  SinkArgs g = sink_bwd_args(a, w);
+  const SinkBwdSizes z = sink_bwd_sizes(g);
+  if (!workspace) return ESA_ERR_NULL;
+  if (!aligned(workspace, 16)) return ESA_ERR_ALIGN;
+  if (workspace_bytes < z.total()) return ESA_ERR_CAPACITY;
+  g.delta = (float*)workspace;
+  g.lse2 = (float*)((char*)workspace + z.stat);
+  g.partial = (float*)((char*)workspace + 2 * z.stat);
+  return launch_sink_bwd(g, (hipStream_t)stream) == hipSuccess ? ESA_OK : ESA_ERR_HIP;
 }
 
 }  // extern "C"

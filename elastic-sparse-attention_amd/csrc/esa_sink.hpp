@@ -1,0 +1,453 @@
+// Attention over a causal sliding window and a few first keys that stay
+// visible (sinks), gfx950: what the forward, backward and decode kernels
+// share.
+//
+// Row r of sequence b sits at position p = base(b) + r; its keys are
+//   f <= j <= p  and  (p - j < window  or  j - f < sinks),   f = first_key(b).
+// The kernels see the pattern as ranges: nothing but these numbers decides
+// which key blocks a row block visits and which keys of a block count.
+#pragma once
+#include "esa_tile.hpp"
+
+namespace esa {
+
+struct SinkArgs {
+  const void *q, *k, *v;
+  void* o;
+  float* lse;
+  const void* dout;
+  void *dq, *dk, *dv;
+  int64_t qsb, qsh, qss, ksb, ksh, kss, vsb, vsh, vss, osb, osh, oss, lsb, lsh;
+  int64_t dosb, dosh, doss, dqsb, dqsh, dqss, dksb, dksh, dkss, dvsb, dvsh, dvss;
+  int B, H, Hkv, groups, q_len, kv_len;
+  int d_real;  // head_dim: dims d_real .. D - 1 of a kernel's D read as zeros
+  int window, sinks;  // (both at most kv_len)
+  const int64_t* pos;  // positions, or NULL (row r is position r)
+  int64_t pos_sb;      // 0: shared by the batch
+  const int64_t* first;  // first keys, or NULL (0)
+  int elem;
+  float sm_scale, scale_log2;
+  int nqb;        // row blocks a head
+  int xcd_runs;   // the grid's workgroups of one XCD take consecutive items
+  // backward
+  float* delta;  // [B, H, qpad] rowsum(dO * O)
+  float* lse2;   // [B, H, qpad] log2(e) * lse
+  int qpad;
+  int nkb, n_sink_blocks;     // 128-key blocks a kv head; the first ones hold sinks
+  int chunks, sink_chunks;    // row chunks of a block, of a sink block
+  float* partial;             // partial sums of blocks with more than one chunk
+  // decode
+  int splits;                 // key ranges a (sequence, kv head, row tile)
+  int row_tiles;              // 16-row tiles of its groups * q_len rows
+  float* part_ml;             // [.., splits, 16] running max and sum
+};
+
+// Where a sequence's rows and keys start.  ok: the first position lies inside
+// the cache.
+struct SeqInfo {
+  int base, first;
+  bool ok;
+};
+__device__ __forceinline__ SeqInfo seq_info(const SinkArgs& A, int b) {
+  SeqInfo s{0, 0, true};
+  if (A.pos) {
+    int64_t p = A.pos[(int64_t)b * A.pos_sb];
+    p += p < 0 ? A.kv_len : 0;
+    s.ok = p >= 0 && p < A.kv_len;
+    s.base = s.ok ? (int)p : 0;
+  }
+  if (A.first) {
+    const int64_t f = A.first[b];
+    s.first = (int)(f < 0 ? 0 : f > A.kv_len ? A.kv_len : f);
+  }
+  return s;
+}
+
+// Row r's own position is base + r, inside the cache (else: a NaN row).
+__device__ __forceinline__ bool row_valid(const SinkArgs& A, const SeqInfo& s, int b, int r) {
+  if (!A.pos) return true;
+  int64_t p = A.pos[(int64_t)b * A.pos_sb + r];
+  p += p < 0 ? A.kv_len : 0;
+  return s.ok && p == (int64_t)s.base + r && p < A.kv_len;
+}
+
+// The keys of [k0, k0 + 32) that the row at position p sees, as bits.
+__device__ __forceinline__ uint32_t seen_keys(int p, int k0, int window, int sink_end) {
+  const uint32_t win = range_word(p - window + 1 - k0, p - k0, 0);
+  return win | range_word(0, min(sink_end - 1, p) - k0, 0);
+}
+// The rows (positions) of [p0, p0 + 32), up to p_last, that see key j, as bits.
+__device__ __forceinline__ uint32_t seen_rows(int j, int p0, int p_last, int window,
+                                              int sink_end) {
+  const int hi = j < sink_end ? p_last : min(p_last, j + window - 1);
+  return range_word(j - p0, hi - p0, 0);
+}
+// Rows [p0, p1] against keys [k0, k0 + 32): is every pair visible, is none?
+__device__ __forceinline__ bool all_seen(int p0, int p1, int k0, int window, int sink_end) {
+  return k0 + 31 <= p0 && (k0 > p1 - window || k0 + 32 <= sink_end);
+}
+__device__ __forceinline__ bool none_seen(int p0, int p1, int k0, int window, int sink_end) {
+  return k0 > p1 || (k0 + 31 <= p0 - window && k0 >= sink_end);
+}
+
+// A row kernel's work item: a kv head's row blocks from the last (the most
+// keys), the query heads that share it next to each other, so that an XCD
+// works on the same keys at a time.
+struct RowItem {
+  int b, kvh, h, qb;
+};
+__device__ __forceinline__ RowItem row_item(const SinkArgs& A) {
+  int item = blockIdx.x;
+  if (A.xcd_runs) item = (item & 7) * ((int)gridDim.x >> 3) + (item >> 3);
+  const int per = A.nqb * A.groups;
+  const int bkv = item / per, rem = item - bkv * per;
+  RowItem it;
+  it.qb = A.nqb - 1 - rem / A.groups;
+  it.b = bkv / A.Hkv;
+  it.kvh = bkv - it.b * A.Hkv;
+  it.h = it.kvh * A.groups + rem % A.groups;
+  return it;
+}
+// Whole kv heads fall to each XCD (workgroup id % 8) where their number allows.
+inline int sink_xcd_runs(const SinkArgs& a, int64_t grid) {
+  return ((int64_t)a.B * a.Hkv) % 8 == 0 && grid % 8 == 0;
+}
+
+// The key stages of 128 rows from r0: n_sink stages of the sinks, then stages
+// from m0 to the last row's position; one run where the two meet.
+struct KeyStages {
+  int f, n_sink, m0, n_all, step;
+  int pb;  // the last row's position, inside the cache
+  __device__ __forceinline__ int key0(int i) const {
+    return i < n_sink ? f + i * step : m0 + (i - n_sink) * step;
+  }
+};
+template <int STAGE>
+__device__ __forceinline__ KeyStages key_stages(const SinkArgs& A, const SeqInfo& si, int r0,
+                                                int sink_end) {
+  KeyStages k;
+  k.step = STAGE;
+  k.f = si.first;
+  k.pb = min(si.base + min(r0 + 127, A.q_len - 1), A.kv_len - 1);
+  const int lo = max(k.f, si.base + r0 - A.window + 1);
+  k.n_sink = lo > k.f && k.pb >= k.f ? (min(sink_end, lo) - k.f + STAGE - 1) / STAGE : 0;
+  k.m0 = lo;
+  if (k.n_sink > 0 && lo <= k.f + k.n_sink * STAGE) {
+    k.n_sink = 0;
+    k.m0 = k.f;
+  }
+  k.n_all = k.n_sink + (k.pb >= k.m0 ? (k.pb - k.m0) / STAGE + 1 : 0);
+  return k;
+}
+
+// ---------------------------------------------------------------------------
+// Products of 32 x 32 blocks of one wave, for 16-bit types and float32.  Each
+// lane owns column l % 32 (a row of q, or a key); hf = l / 32.
+//   row_product   S[i][col] = sum_d X[i][d] col[d]: X's rows from LDS as the A
+//                 operand, the lane's own row (Frag) as B
+//   col_product   Y^T[d][col] += sum_i X[i][d] P[i][col]: the same LDS rows
+//                 read by columns; P straight from a product's accumulators
+// Accumulator register r of lane half hf is row 8 (r / 4) + 4 hf + r % 4.
+// LDS rows are D elements unpadded, their 16-byte chunks XOR-swizzled by the
+// row, so that both kinds of read meet each bank once.
+template <int D, Elem E>
+struct SinkTile {
+  using M = MmaT<E>;
+  using V8 = typename M::v8;
+  static constexpr int ES = 2;
+  static constexpr int EPC = 8;        // elements of a chunk
+  static constexpr int NS = D / 16, ND = D / 32;
+  static constexpr int CPR = D / 8;    // chunks of a row
+  struct Frag {
+    V8 f[NS];
+  };
+  struct P {
+    uint32_t w[8];
+  };
+  using LdsT = uint16_t;
+  static constexpr uint32_t kOne = E == Elem::bf16 ? 0x3F80u : 0x3C00u;
+
+  int ra[NS];  // element offsets of a 32-row block's row reads
+  int ca[ND];  // ... of its column reads, rows 4 hf + 0 .. 3 (+ 16 u)
+  int hf;
+
+  static __device__ __forceinline__ int swz(int row) { return swz_k<(D >= 128 ? 128 : 64)>(row); }
+  __device__ __forceinline__ void init(int lane) {
+    hf = lane >> 5;
+    const int l32 = lane & 31, g4 = lane >> 4, lam = lane & 15;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) ra[s] = l32 * D + 8 * ((2 * s + hf) ^ swz(l32));
+    const int row = 4 * hf + (lam >> 2);
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      const int col = 32 * d + 16 * (g4 & 1) + 4 * (lam & 3);
+      ca[d] = row * D + 8 * ((col >> 3) ^ swz(row)) + (col & 7);
+    }
+  }
+  __device__ __forceinline__ void load_frag(Frag& f, const void* row, bool ok, int d_real) const {
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      u32x4 raw = {0u, 0u, 0u, 0u};
+      const int d = 16 * s + 8 * hf;
+      if (ok && d < d_real) raw = *(const u32x4*)((const uint16_t*)row + d);
+      f.f[s] = __builtin_bit_cast(V8, raw);
+    }
+  }
+  __device__ __forceinline__ void row_product(f32x16& acc, const LdsT* buf, int rb,
+                                              const Frag& f) const {
+    V8 a[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) a[s] = *(const V8*)(buf + ra[s] + 32 * rb * D);
+#pragma unroll
+    for (int s = 0; s < NS; ++s) acc = M::mfma32(a[s], f.f[s], acc);
+  }
+  __device__ __forceinline__ P pack(const f32x16& v) const {
+    P p;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) p.w[q] = M::pack2(v[2 * q], v[2 * q + 1]);
+    return p;
+  }
+  // the A operand of dims 32 d .. and rows 16 u .. of block rb, by columns
+  __device__ __forceinline__ u32x4 col_operand(const LdsT* buf, int rb, int d, int u) const {
+    const LdsT* p1 = buf + ca[d] + (32 * rb + 16 * u) * D;
+    const LdsT* p2 = buf + (ca[d] ^ 16) + (32 * rb + 16 * u + 8) * D;
+    const s16x4 v[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p1),
+                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p2)};
+    return __builtin_bit_cast(u32x4, v);
+  }
+  __device__ __forceinline__ void col_product(f32x16 (&acc)[ND], const LdsT* buf, int rb,
+                                              const P& p) const {
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const u32x4 a = col_operand(buf, rb, d, u);
+        const u32x4 b = {p.w[4 * u], p.w[4 * u + 1], p.w[4 * u + 2], p.w[4 * u + 3]};
+        acc[d] = M::mfma32(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), acc[d]);
+      }
+  }
+  // dims 32 d + 8 q4 + 4 hf .. of the lane's own row
+  static __device__ __forceinline__ void store4(void* row, int dim, float a, float b, float c,
+                                                float e) {
+    typename M::v4 v;
+    v[0] = (typename M::s)a;
+    v[1] = (typename M::s)b;
+    v[2] = (typename M::s)c;
+    v[3] = (typename M::s)e;
+    *(typename M::v4*)((uint16_t*)row + dim) = v;
+  }
+  static __device__ __forceinline__ float psum(const P& p, float c) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) c = M::dot2(p.w[q], c);
+    return c;
+  }
+};
+
+template <int D>
+struct SinkTile<D, Elem::f32> {
+  static constexpr int ES = 4;
+  static constexpr int EPC = 4;
+  static constexpr int NU = D / 8, ND = D / 32;
+  static constexpr int CPR = D / 4;
+  struct Frag {
+    f32x4 f[NU];
+  };
+  using P = f32x16;
+  using LdsT = float;
+
+  int ra;     // row reads: the lane's row; chunk 2 u + hf is XORed in below
+  int sw;
+  int ca[4];  // column reads of rows 4 hf + t
+  int hf;
+
+  static __device__ __forceinline__ int swz(int row) { return row & 7; }
+  __device__ __forceinline__ void init(int lane) {
+    hf = lane >> 5;
+    const int l32 = lane & 31;
+    ra = l32 * D;
+    sw = l32 & 7;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int row = 4 * hf + t;
+      ca[t] = row * D + 4 * ((l32 >> 2) ^ row) + (l32 & 3);
+    }
+  }
+  __device__ __forceinline__ void load_frag(Frag& f, const void* row, bool ok, int d_real) const {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      f32x4 raw = {0.f, 0.f, 0.f, 0.f};
+      const int d = 8 * u + 4 * hf;
+      if (ok && d < d_real) raw = *(const f32x4*)((const float*)row + d);
+      f.f[u] = raw;
+    }
+  }
+  __device__ __forceinline__ void row_product(f32x16& acc, const float* buf, int rb,
+                                              const Frag& f) const {
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const f32x4 a = *(const f32x4*)(buf + ra + 32 * rb * D + 4 * ((2 * u + hf) ^ sw));
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[t], f.f[u][t], acc, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ P pack(const f32x16& v) const { return v; }
+  __device__ __forceinline__ float col_operand(const float* buf, int rb, int d, int r) const {
+    return buf[ca[r & 3] + (32 * rb + 8 * (r >> 2)) * D + 32 * d];
+  }
+  __device__ __forceinline__ void col_product(f32x16 (&acc)[ND], const float* buf, int rb,
+                                              const P& p) const {
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(col_operand(buf, rb, d, r), p[r], acc[d], 0,
+                                                      0, 0);
+  }
+  static __device__ __forceinline__ void store4(void* row, int dim, float a, float b, float c,
+                                                float e) {
+    *(f32x4*)((float*)row + dim) = f32x4{a, b, c, e};
+  }
+  static __device__ __forceinline__ float psum(const P& p, float c) {
+#pragma unroll
+    for (int q = 0; q < 16; ++q) c += p[q];
+    return c;
+  }
+};
+
+// ROWS rows of D elements from one matrix into LDS, 16 bytes a lane and load:
+// the buffer resource starts at the stage's first row (so a row's offset stays
+// small however long the tensor is) and ends with the last row; whatever lies
+// past it, or past head_dim, reads as zero.
+template <int D, Elem E, int ROWS, int THREADS>
+struct SinkStage {
+  using T = SinkTile<D, E>;
+  static constexpr int LOADS = ROWS * T::CPR / THREADS;
+  static constexpr int BYTES = ROWS * D * T::ES;
+  static_assert(LOADS >= 1 && LOADS * THREADS == ROWS * T::CPR, "whole stage per load round");
+  int off[LOADS];
+  const char* base;
+  int64_t stride;  // bytes
+  int rows;        // rows of the matrix
+  int row_bytes;
+
+  __device__ __forceinline__ void init(const void* p, int64_t stride_elems, int n_rows, int d_real,
+                                       int tid) {
+    base = (const char*)p;
+    stride = stride_elems * T::ES;
+    rows = n_rows;
+    row_bytes = d_real * T::ES;
+    const int lane = tid & 63, wave = tid >> 6;
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+      const int slot = (LOADS * wave + j) * 64 + lane;
+      const int row = slot / T::CPR, chunk = (slot % T::CPR) ^ T::swz(row);
+      off[j] = 16 * chunk < row_bytes ? (int)(row * stride) + 16 * chunk : 0x7ffffff0;
+    }
+  }
+  // rows row0 .. row0 + ROWS - 1 -> dst
+  __device__ __forceinline__ void issue(int row0, void* dst, int wave) const {
+    const int64_t left = (int64_t)(rows - row0 - 1) * stride + row_bytes;
+    const int n = rows > row0 ? (int)(left < 0x7fffff00 ? left : 0x7fffff00) : 0;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)(base + (int64_t)row0 * stride), (short)0, n, 0x00020000);
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j)
+      load_lds16(rs, (uint16_t*)dst + (LOADS * wave + j) * 512, off[j], 0);
+  }
+};
+
+// Waits for this wave's loads into LDS, then for the other waves' (and for
+// their reads of the buffer that is filled next).
+__device__ __forceinline__ void stage_ready() {
+  __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
+  __syncthreads();
+}
+
+// Non-finite values.  A staged block also holds rows that a column does not
+// see; they meet P = 0 in the products, and 0 * Inf is NaN (so is the mask's
+// -inf plus an Inf score).  The kernels therefore look at what they stored:
+// a row (or key) whose values came out non-finite is computed again from the
+// pairs that it sees alone, by one wave in float32, so a hidden Inf or NaN
+// reaches nothing and a visible one exactly what the formula gives.
+//
+// The keys of one row in order: n_sink sinks from f, then lo .. p.
+struct RowKeys {
+  int f, n_sink, lo, n;
+  __device__ __forceinline__ int key(int i) const { return i < n_sink ? f + i : lo + i - n_sink; }
+};
+__device__ __forceinline__ RowKeys row_keys(int p, int f, int window, int sink_end) {
+  RowKeys k;
+  k.f = f;
+  k.lo = max(f, p - window + 1);
+  k.n_sink = max(0, min(sink_end, k.lo) - f);
+  k.n = p < f ? 0 : k.n_sink + p - k.lo + 1;
+  return k;
+}
+
+// sum_d a[d] b[d] over d_real elements (whole 16-byte chunks)
+template <Elem E>
+__device__ __forceinline__ float row_dot(const void* a, const void* b, int d_real) {
+  using T = ElemT<E>;
+  float s = 0.f;
+#pragma unroll 1
+  for (int d = 0; d < d_real; d += T::kPerChunk) {
+    const u32x4 x = *(const u32x4*)((const typename T::T*)a + d);
+    const u32x4 y = *(const u32x4*)((const typename T::T*)b + d);
+#pragma unroll
+    for (int e = 0; e < T::kPerChunk; ++e) s = __builtin_fmaf(T::chunk(x, e), T::chunk(y, e), s);
+  }
+  return s;
+}
+
+// Row `row` of one head from its own keys, by one wave: lanes take 64 keys at a
+// time for the scores and the head's dims for the weighted sum.
+template <Elem E>
+__device__ void fix_row(const SinkArgs& A, int b, int h, int kvh, int row, int p, int f,
+                        int sink_end, int lane) {
+  using T = ElemT<E>;
+  using EL = typename T::T;
+  const EL* q = (const EL*)A.q + (int64_t)b * A.qsb + (int64_t)h * A.qsh + (int64_t)row * A.qss;
+  const EL* k = (const EL*)A.k + (int64_t)b * A.ksb + (int64_t)kvh * A.ksh;
+  const EL* v = (const EL*)A.v + (int64_t)b * A.vsb + (int64_t)kvh * A.vsh;
+  const RowKeys rk = row_keys(p, f, A.window, sink_end);
+  float m = -INFINITY, l = 0.f, acc[2] = {0.f, 0.f};
+#pragma unroll 1
+  for (int i0 = 0; i0 < rk.n; i0 += 64) {
+    const bool in = i0 + lane < rk.n;
+    float s = -INFINITY;
+    if (in)
+      s = row_dot<E>(q, k + (int64_t)rk.key(i0 + lane) * A.kss, A.d_real) * A.scale_log2;
+    const float top = fmaxf(m, wave_max(s)), use = top == -INFINITY ? 0.f : top;
+    const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - use);
+    const float pr = in ? __builtin_amdgcn_exp2f(s - use) : 0.f;
+    m = top;
+    l = l * alpha + wave_sum(pr);
+    acc[0] *= alpha;
+    acc[1] *= alpha;
+    const int n = min(64, rk.n - i0);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const float w = __shfl(pr, i, 64);
+      const EL* vr = v + (int64_t)rk.key(i0 + i) * A.vss;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        if (lane + 64 * c < A.d_real)
+          acc[c] = __builtin_fmaf(w, T::load(vr + lane + 64 * c), acc[c]);
+    }
+  }
+  const bool empty = rk.n <= 0;
+  EL* o = (EL*)A.o + (int64_t)b * A.osb + (int64_t)h * A.osh + (int64_t)row * A.oss;
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+    if (lane + 64 * c < A.d_real) T::store(o + lane + 64 * c, empty ? 0.f : acc[c] / l);
+  if (A.lse && lane == 0)
+    A.lse[(int64_t)b * A.lsb + (int64_t)h * A.lsh + row] =
+        empty ? -INFINITY : (m + __log2f(l)) * 0.69314718055994530942f;
+}
+
+hipError_t launch_sink_fwd(const SinkArgs& a, hipStream_t stream);
+hipError_t launch_sink_bwd(const SinkArgs& a, hipStream_t stream);
+hipError_t launch_sink_decode(const SinkArgs& a, hipStream_t stream);
+
+}  // namespace esa

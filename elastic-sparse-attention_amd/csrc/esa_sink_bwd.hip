@@ -1,0 +1,571 @@
+// Backward of attention over a causal window with sinks (gfx950), without
+// atomics: every gradient is summed in a fixed order.
+//
+//   P = exp(scale s - lse),  dV = P^T dO,  dP = dO V^T,
+//   dS = P * (dP - delta),  delta = rowsum(dO * O),
+//   dQ = scale dS K,  dK = scale dS^T Q
+//
+//   sink_prep_kernel  delta and lse in log2 units, one 16-lane group a row
+//   sink_dq_kernel    128 rows a workgroup, over the keys they see, as the
+//                     forward: S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T
+//   sink_dkdv_kernel  128 keys a workgroup, over the rows that see them: the
+//                     lane's own key row (K, V) in registers, rows of Q and dO
+//                     staged in LDS: S = Q K^T, dP = dO V^T, dV^T += dO^T P,
+//                     dK^T += Q^T dS
+//   sink_join_kernel  blocks whose rows were split: the parts in order
+//
+// Key blocks start at the sequence's first key, so the sinks are in the first
+// ones.  A sink is seen by every later row: its block's rows (all query heads
+// of the kv group, one after the other) are cut into `sink_chunks` workgroups
+// of about a window block's rows each, which leave float32 parts; other blocks
+// are cut into `chunks` where the grid alone would not fill the chip.
+#include <algorithm>
+
+#include "esa_sink.hpp"
+
+namespace esa {
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int D, Elem E>
+struct SinkBwdCfg {
+  static constexpr int STAGE = E == Elem::f32 ? 32 : 64;  // keys (dQ) or rows (dK / dV)
+  static constexpr int NB = STAGE / 32;
+  static constexpr int WAVES_PER_SIMD = E == Elem::f32 ? 1 : 2;
+};
+
+template <Elem E>
+__device__ __forceinline__ const typename ElemT<E>::T* at(const void* p, int64_t off) {
+  return (const typename ElemT<E>::T*)p + off;
+}
+
+template <Elem E>
+__global__ __launch_bounds__(256) void sink_prep_kernel(SinkArgs A) {
+  using T = ElemT<E>;
+  const int g = threadIdx.x & 15;
+  const int64_t rows = (int64_t)A.B * A.H * A.q_len;
+  for (int64_t id = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); id < rows;
+       id += (int64_t)gridDim.x * 16) {
+    const int64_t bh = id / A.q_len;
+    const int r = (int)(id - bh * A.q_len);
+    const int b = (int)(bh / A.H), h = (int)(bh - (int64_t)b * A.H);
+    const auto* o = at<E>(A.o, (int64_t)b * A.osb + (int64_t)h * A.osh + (int64_t)r * A.oss);
+    const auto* d = at<E>(A.dout, (int64_t)b * A.dosb + (int64_t)h * A.dosh + (int64_t)r * A.doss);
+    float acc = 0.f;
+    for (int c = g * T::kPerChunk; c < A.d_real; c += 16 * T::kPerChunk) {
+      const u32x4 x = *(const u32x4*)(o + c), y = *(const u32x4*)(d + c);
+#pragma unroll
+      for (int e = 0; e < T::kPerChunk; ++e) acc = __builtin_fmaf(T::chunk(x, e), T::chunk(y, e), acc);
+    }
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) acc += __shfl_xor(acc, off, 16);
+    if (g == 0) {
+      const float lse = A.lse[(int64_t)b * A.lsb + (int64_t)h * A.lsh + r];
+      A.delta[bh * A.qpad + r] = acc;
+      // a row that sees nothing: kept finite, so its masked scores give P = 0
+      A.lse2[bh * A.qpad + r] = lse == -INFINITY ? -3.0e38f : lse * kLog2e;
+    }
+  }
+}
+
+// dQ of one row from its own keys, by one wave
+template <Elem E>
+__device__ void fix_dq_row(const SinkArgs& A, int b, int h, int kvh, int row, int p, int f,
+                           int sink_end, int lane) {
+  using T = ElemT<E>;
+  const auto* q = at<E>(A.q, (int64_t)b * A.qsb + (int64_t)h * A.qsh + (int64_t)row * A.qss);
+  const auto* g = at<E>(A.dout, (int64_t)b * A.dosb + (int64_t)h * A.dosh + (int64_t)row * A.doss);
+  const auto* k = at<E>(A.k, (int64_t)b * A.ksb + (int64_t)kvh * A.ksh);
+  const auto* v = at<E>(A.v, (int64_t)b * A.vsb + (int64_t)kvh * A.vsh);
+  const int64_t st = ((int64_t)b * A.H + h) * A.qpad + row;
+  const float lse2 = A.lse2[st], delta = A.delta[st];
+  const RowKeys rk = row_keys(p, f, A.window, sink_end);
+  float acc[2] = {0.f, 0.f};
+#pragma unroll 1
+  for (int i0 = 0; i0 < rk.n; i0 += 64) {
+    float ds = 0.f;
+    if (i0 + lane < rk.n) {
+      const int64_t j = rk.key(i0 + lane);
+      const float s = row_dot<E>(q, k + j * A.kss, A.d_real) * A.scale_log2;
+      const float dp = row_dot<E>(g, v + j * A.vss, A.d_real);
+      ds = __builtin_amdgcn_exp2f(s - lse2) * (dp - delta) * A.sm_scale;
+    }
+    const int n = min(64, rk.n - i0);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      const float w = __shfl(ds, i, 64);
+      const auto* kr = k + (int64_t)rk.key(i0 + i) * A.kss;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        if (lane + 64 * c < A.d_real)
+          acc[c] = __builtin_fmaf(w, T::load(kr + lane + 64 * c), acc[c]);
+    }
+  }
+  auto* dq = (typename T::T*)A.dq + (int64_t)b * A.dqsb + (int64_t)h * A.dqsh + (int64_t)row * A.dqss;
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+    if (lane + 64 * c < A.d_real) T::store(dq + lane + 64 * c, acc[c]);
+}
+
+template <int D, Elem E>
+__global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_dq_kernel(
+    SinkArgs A) {
+  using C = SinkBwdCfg<D, E>;
+  using T = SinkTile<D, E>;
+  using Stage = SinkStage<D, E, C::STAGE, 256>;
+  using LdsT = typename T::LdsT;
+  constexpr int ND = T::ND;
+  __shared__ __attribute__((aligned(1024))) LdsT k_st0[C::STAGE * D];
+  __shared__ __attribute__((aligned(1024))) LdsT v_st0[C::STAGE * D];
+  __shared__ __attribute__((aligned(1024))) LdsT k_st1[C::STAGE * D];
+  __shared__ __attribute__((aligned(1024))) LdsT v_st1[C::STAGE * D];
+
+  const RowItem it = row_item(A);
+  const int b = it.b, h = it.h, kvh = it.kvh, r0 = it.qb * 128;
+  const SeqInfo si = seq_info(A, b);
+  const int f = si.first, sink_end = min(f + A.sinks, A.kv_len), W = A.window;
+  const KeyStages keys = key_stages<C::STAGE>(A, si, r0, sink_end);
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hf = lane >> 5;
+  const int r = r0 + wave * 32 + l32;
+  const bool row_in = r < A.q_len;
+  const int p = si.base + r;
+  const int pb = keys.pb, pw0 = si.base + r0 + wave * 32, pw1 = min(pw0 + 31, pb);
+
+  T t;
+  t.init(lane);
+  typename T::Frag qf, gf;
+  t.load_frag(qf, at<E>(A.q, (int64_t)b * A.qsb + (int64_t)h * A.qsh + (int64_t)r * A.qss), row_in,
+              A.d_real);
+  t.load_frag(gf, at<E>(A.dout, (int64_t)b * A.dosb + (int64_t)h * A.dosh + (int64_t)r * A.doss),
+              row_in, A.d_real);
+  const int64_t st = ((int64_t)b * A.H + h) * A.qpad + r;
+  const float lse2 = row_in ? A.lse2[st] : 0.f, delta = row_in ? A.delta[st] : 0.f;
+  f32x16 acc[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
+  const float scale = A.scale_log2;
+
+  Stage ks, vs;
+  ks.init(at<E>(A.k, (int64_t)b * A.ksb + (int64_t)kvh * A.ksh), A.kss, A.kv_len, A.d_real, tid);
+  vs.init(at<E>(A.v, (int64_t)b * A.vsb + (int64_t)kvh * A.vsh), A.vss, A.kv_len, A.d_real, tid);
+
+  auto block = [&](const LdsT* kbuf, const LdsT* vbuf, int kb, int k0)
+                   __attribute__((always_inline)) {
+    if (pw0 > pb || none_seen(pw0, pw1, k0, W, sink_end)) return;
+    f32x16 s = f32x16{}, dp = f32x16{};
+    if (!all_seen(pw0, pw0 + 31, k0, W, sink_end))
+      mask_init<0>(s, ~(seen_keys(p, k0, W, sink_end) >> (4 * hf)));
+    t.row_product(s, kbuf, kb, qf);
+    t.row_product(dp, vbuf, kb, gf);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -lse2)) * (dp[i] - delta);
+    t.col_product(acc, kbuf, kb, t.pack(s));
+  };
+  auto stage = [&](const LdsT* kbuf, const LdsT* vbuf, int i) __attribute__((always_inline)) {
+    const int k0 = keys.key0(i);
+#pragma unroll
+    for (int kb = 0; kb < C::NB; ++kb) block(kbuf, vbuf, kb, k0 + 32 * kb);
+  };
+  const int n_all = keys.n_all;
+  if (n_all > 0) {
+    ks.issue(keys.key0(0), k_st0, wave);
+    vs.issue(keys.key0(0), v_st0, wave);
+  }
+  for (int i = 0; i < n_all; i += 2) {
+    stage_ready();
+    if (i + 1 < n_all) {
+      ks.issue(keys.key0(i + 1), k_st1, wave);
+      vs.issue(keys.key0(i + 1), v_st1, wave);
+    }
+    stage(k_st0, v_st0, i);
+    if (i + 1 >= n_all) break;
+    stage_ready();
+    if (i + 2 < n_all) {
+      ks.issue(keys.key0(i + 2), k_st0, wave);
+      vs.issue(keys.key0(i + 2), v_st0, wave);
+    }
+    stage(k_st1, v_st1, i + 1);
+  }
+
+  const bool met = row_in && !sum_finite(acc);
+  if (row_in) {
+    auto* row = (typename ElemT<E>::T*)A.dq + (int64_t)b * A.dqsb + (int64_t)h * A.dqsh +
+                (int64_t)r * A.dqss;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4) {
+        const int dim = 32 * d + 8 * q4 + 4 * hf;
+        if (dim < A.d_real)
+          T::store4(row, dim, acc[d][4 * q4] * A.sm_scale, acc[d][4 * q4 + 1] * A.sm_scale,
+                    acc[d][4 * q4 + 2] * A.sm_scale, acc[d][4 * q4 + 3] * A.sm_scale);
+      }
+  }
+  uint64_t bad = __builtin_amdgcn_ballot_w64(met);
+  bad = (bad | bad >> 32) & 0xffffffffull;
+  if (bad) __builtin_amdgcn_s_waitcnt(0);  // the stores above come first
+  while (bad) {
+    const int i = __builtin_ctzll(bad);
+    bad &= bad - 1;
+    const int row = r0 + wave * 32 + i;
+    fix_dq_row<E>(A, b, h, kvh, row, min(si.base + row, A.kv_len - 1), f, sink_end, lane);
+  }
+}
+
+// One key block's work: which rows, how they are cut.
+struct KeyItem {
+  int b, kvh, kblk, chunk, n_chunks;
+  int64_t part;  // index of its float32 part
+};
+__device__ __forceinline__ KeyItem key_item(const SinkArgs& A, int item) {
+  const int n_reg = A.nkb - A.n_sink_blocks;
+  const int units = A.n_sink_blocks * A.sink_chunks + n_reg * A.chunks;
+  const int bkv = item / units;
+  int u = item - bkv * units;
+  KeyItem k;
+  k.b = bkv / A.Hkv;
+  k.kvh = bkv - k.b * A.Hkv;
+  const int n_sink_units = A.n_sink_blocks * A.sink_chunks;
+  if (u < n_sink_units) {
+    k.kblk = u / A.sink_chunks;
+    k.chunk = u - k.kblk * A.sink_chunks;
+    k.n_chunks = A.sink_chunks;
+  } else {
+    const int w = u - n_sink_units;
+    k.kblk = w / A.chunks;
+    k.chunk = w - k.kblk * A.chunks;
+    k.n_chunks = A.chunks;
+    k.kblk += A.n_sink_blocks;
+  }
+  k.part = (int64_t)bkv * (A.n_sink_blocks * A.sink_chunks + (A.chunks > 1 ? n_reg * A.chunks : 0)) +
+           u;
+  return k;
+}
+
+// Stores 32 keys' dK^T and dV^T (one wave's accumulators)
+template <int D, Elem E>
+__device__ __forceinline__ void store_keys(const SinkArgs& A, int b, int kvh, int j, int hf,
+                                           const f32x16 (&dk)[SinkTile<D, E>::ND],
+                                           const f32x16 (&dv)[SinkTile<D, E>::ND]) {
+  using T = SinkTile<D, E>;
+  auto* kr = (typename ElemT<E>::T*)A.dk + (int64_t)b * A.dksb + (int64_t)kvh * A.dksh +
+             (int64_t)j * A.dkss;
+  auto* vr = (typename ElemT<E>::T*)A.dv + (int64_t)b * A.dvsb + (int64_t)kvh * A.dvsh +
+             (int64_t)j * A.dvss;
+  const float c = A.sm_scale;
+#pragma unroll
+  for (int d = 0; d < T::ND; ++d)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      const int dim = 32 * d + 8 * q4 + 4 * hf;
+      if (dim < A.d_real) {
+        T::store4(kr, dim, dk[d][4 * q4] * c, dk[d][4 * q4 + 1] * c, dk[d][4 * q4 + 2] * c,
+                  dk[d][4 * q4 + 3] * c);
+        T::store4(vr, dim, dv[d][4 * q4], dv[d][4 * q4 + 1], dv[d][4 * q4 + 2],
+                  dv[d][4 * q4 + 3]);
+      }
+    }
+}
+
+// dK and dV of one key from the rows that see it, by one wave
+template <Elem E>
+__device__ void fix_key(const SinkArgs& A, const SeqInfo& si, int b, int kvh, int j, int sink_end,
+                        int lane) {
+  using T = ElemT<E>;
+  const auto* k = at<E>(A.k, (int64_t)b * A.ksb + (int64_t)kvh * A.ksh + (int64_t)j * A.kss);
+  const auto* v = at<E>(A.v, (int64_t)b * A.vsb + (int64_t)kvh * A.vsh + (int64_t)j * A.vss);
+  const int p_last = min(si.base + A.q_len, A.kv_len) - 1;
+  const int hi = j < sink_end ? p_last : min(p_last, j + A.window - 1);
+  const int lo = max(j, si.base);
+  float ak[2] = {0.f, 0.f}, av[2] = {0.f, 0.f};
+#pragma unroll 1
+  for (int h = kvh * A.groups; h < (kvh + 1) * A.groups; ++h) {
+    const auto* q = at<E>(A.q, (int64_t)b * A.qsb + (int64_t)h * A.qsh);
+    const auto* g = at<E>(A.dout, (int64_t)b * A.dosb + (int64_t)h * A.dosh);
+    const int64_t st = ((int64_t)b * A.H + h) * A.qpad;
+#pragma unroll 1
+    for (int p0 = lo; p0 <= hi; p0 += 64) {
+      float pr = 0.f, ds = 0.f;
+      if (p0 + lane <= hi) {
+        const int64_t r = p0 + lane - si.base;
+        const float s = row_dot<E>(q + r * A.qss, k, A.d_real) * A.scale_log2;
+        const float dp = row_dot<E>(g + r * A.doss, v, A.d_real);
+        pr = __builtin_amdgcn_exp2f(s - A.lse2[st + r]);
+        ds = pr * (dp - A.delta[st + r]) * A.sm_scale;
+      }
+      const int n = min(64, hi - p0 + 1);
+#pragma unroll 1
+      for (int i = 0; i < n; ++i) {
+        const float wp = __shfl(pr, i, 64), wd = __shfl(ds, i, 64);
+        const int64_t r = p0 + i - si.base;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+          if (lane + 64 * c < A.d_real) {
+            ak[c] = __builtin_fmaf(wd, T::load(q + r * A.qss + lane + 64 * c), ak[c]);
+            av[c] = __builtin_fmaf(wp, T::load(g + r * A.doss + lane + 64 * c), av[c]);
+          }
+      }
+    }
+  }
+  auto* kr = (typename T::T*)A.dk + (int64_t)b * A.dksb + (int64_t)kvh * A.dksh + (int64_t)j * A.dkss;
+  auto* vr = (typename T::T*)A.dv + (int64_t)b * A.dvsb + (int64_t)kvh * A.dvsh + (int64_t)j * A.dvss;
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+    if (lane + 64 * c < A.d_real) {
+      T::store(kr + lane + 64 * c, ak[c]);
+      T::store(vr + lane + 64 * c, av[c]);
+    }
+}
+
+// The keys of a wave whose sums came out non-finite, again (j0: its first key)
+template <Elem E>
+__device__ __forceinline__ void fix_keys(const SinkArgs& A, const SeqInfo& si, int b, int kvh,
+                                         int j0, int sink_end, bool met, int lane) {
+  uint64_t bad = __builtin_amdgcn_ballot_w64(met);
+  bad = (bad | bad >> 32) & 0xffffffffull;
+  if (bad) __builtin_amdgcn_s_waitcnt(0);  // the stores above come first
+  while (bad) {
+    const int i = __builtin_ctzll(bad);
+    bad &= bad - 1;
+    fix_key<E>(A, si, b, kvh, j0 + i, sink_end, lane);
+  }
+}
+
+template <int D, Elem E>
+__global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_dkdv_kernel(
+    SinkArgs A) {
+  using C = SinkBwdCfg<D, E>;
+  using T = SinkTile<D, E>;
+  using Stage = SinkStage<D, E, C::STAGE, 256>;
+  using LdsT = typename T::LdsT;
+  constexpr int ND = T::ND;
+  __shared__ __attribute__((aligned(1024))) LdsT q_st0[C::STAGE * D];
+  __shared__ __attribute__((aligned(1024))) LdsT g_st0[C::STAGE * D];
+  __shared__ __attribute__((aligned(1024))) LdsT q_st1[C::STAGE * D];
+  __shared__ __attribute__((aligned(1024))) LdsT g_st1[C::STAGE * D];
+  __shared__ __attribute__((aligned(256))) float stat0[2 * 64];  // lse2, then delta
+  __shared__ __attribute__((aligned(256))) float stat1[2 * 64];
+
+  int item = blockIdx.x;
+  if (A.xcd_runs) item = (item & 7) * ((int)gridDim.x >> 3) + (item >> 3);
+  const KeyItem it = key_item(A, item);
+  const int b = it.b, kvh = it.kvh;
+  const SeqInfo si = seq_info(A, b);
+  const int f = si.first, sink_end = min(f + A.sinks, A.kv_len), W = A.window;
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l32 = lane & 31, hf = lane >> 5;
+
+  // keys before the sequence's first one: no row sees them
+  if (it.chunk == 0) {
+    const int z1 = min(f, min(it.kblk * 128 + 128, A.kv_len));
+    for (int j = it.kblk * 128 + (tid >> 4); j < z1; j += 16) {
+      auto* kr = (typename ElemT<E>::T*)A.dk + (int64_t)b * A.dksb + (int64_t)kvh * A.dksh +
+                 (int64_t)j * A.dkss;
+      auto* vr = (typename ElemT<E>::T*)A.dv + (int64_t)b * A.dvsb + (int64_t)kvh * A.dvsh +
+                 (int64_t)j * A.dvss;
+      for (int d = 4 * (tid & 15); d < A.d_real; d += 64) {
+        T::store4(kr, d, 0.f, 0.f, 0.f, 0.f);
+        T::store4(vr, d, 0.f, 0.f, 0.f, 0.f);
+      }
+    }
+  }
+  const int j0 = f + it.kblk * 128;
+  if (j0 >= A.kv_len) return;
+
+  // ---- the rows that see the block, as stages of every query head in turn;
+  // this workgroup's share of them
+  const int p_last = min(si.base + A.q_len, A.kv_len) - 1;
+  const int p_lo = max(j0, si.base);
+  const int p_hi = j0 < sink_end ? p_last : min(p_last, j0 + 127 + W - 1);
+  const int per_head = p_hi >= p_lo ? (p_hi - p_lo) / C::STAGE + 1 : 0;
+  const int64_t total = (int64_t)per_head * A.groups;
+  const int s0 = (int)(total * it.chunk / it.n_chunks);
+  const int s1 = (int)(total * (it.chunk + 1) / it.n_chunks);
+
+  const int jw0 = j0 + wave * 32;  // the wave's first key
+  const int j = jw0 + l32;
+  const bool key_in = j < A.kv_len;
+
+  T t;
+  t.init(lane);
+  typename T::Frag kf, vf;
+  t.load_frag(kf, at<E>(A.k, (int64_t)b * A.ksb + (int64_t)kvh * A.ksh + (int64_t)j * A.kss),
+              key_in, A.d_real);
+  t.load_frag(vf, at<E>(A.v, (int64_t)b * A.vsb + (int64_t)kvh * A.vsh + (int64_t)j * A.vss),
+              key_in, A.d_real);
+  f32x16 dk[ND], dv[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
+  const float scale = A.scale_log2;
+
+  Stage qs, gs;
+  qs.init(nullptr, A.qss, A.q_len, A.d_real, tid);
+  gs.init(nullptr, A.doss, A.q_len, A.d_real, tid);
+  int head = per_head > 0 ? s0 / per_head : 0, at_stage = s0 - head * per_head;
+  // the next stage in order -> buffers; returns its first row
+  auto issue = [&](LdsT* qd, LdsT* gd, float* stat) __attribute__((always_inline)) {
+    const int h = kvh * A.groups + head;
+    const int row0 = p_lo - si.base + at_stage * C::STAGE;
+    qs.base = (const char*)at<E>(A.q, (int64_t)b * A.qsb + (int64_t)h * A.qsh);
+    gs.base = (const char*)at<E>(A.dout, (int64_t)b * A.dosb + (int64_t)h * A.dosh);
+    qs.issue(row0, qd, wave);
+    gs.issue(row0, gd, wave);
+    // lse2 and delta, 64 rows each, zeros past q_len: copied to LDS like the
+    // rows, so the whole issue runs without a divergent branch (a branch here
+    // had the compiler save a value for all lanes under the branch's mask)
+    if (wave < 2) {
+      const float* src = (wave ? A.delta : A.lse2) + ((int64_t)b * A.H + h) * A.qpad;
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)src, (short)0, A.q_len * 4, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(stat + wave * 64), 4, lane * 4,
+                                               row0 * 4, 0, 0);
+    }
+    if (++at_stage == per_head) {
+      at_stage = 0;
+      ++head;
+    }
+    return row0;
+  };
+  auto block = [&](const LdsT* qb, const LdsT* gb, const float* stat, int rb, int row0)
+                   __attribute__((always_inline)) {
+    const int p0 = si.base + row0 + 32 * rb, p1 = min(p0 + 31, p_last);
+    if (p0 > p_last || none_seen(p0, p1, jw0, W, sink_end)) return;
+    f32x16 s = f32x16{}, dp = f32x16{};
+    if (p0 + 31 > p_last || !all_seen(p0, p0 + 31, jw0, W, sink_end))
+      mask_init<0>(s, ~(seen_rows(j, p0, p_last, W, sink_end) >> (4 * hf)));
+    t.row_product(s, qb, rb, kf);
+    f32x4 l2[4], dl[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      l2[q] = *(const f32x4*)(stat + 32 * rb + 8 * q + 4 * hf);
+      dl[q] = *(const f32x4*)(stat + 64 + 32 * rb + 8 * q + 4 * hf);
+    }
+    t.row_product(dp, gb, rb, vf);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -l2[i / 4][i % 4]));
+      dp[i] = s[i] * (dp[i] - dl[i / 4][i % 4]);
+    }
+    t.col_product(dv, gb, rb, t.pack(s));
+    t.col_product(dk, qb, rb, t.pack(dp));
+  };
+  int row_a = 0, row_b = 0;
+  if (s0 < s1) row_a = issue(q_st0, g_st0, stat0);
+  for (int i = s0; i < s1; i += 2) {
+    stage_ready();
+    if (i + 1 < s1) row_b = issue(q_st1, g_st1, stat1);
+#pragma unroll
+    for (int rb = 0; rb < C::NB; ++rb) block(q_st0, g_st0, stat0, rb, row_a);
+    if (i + 1 >= s1) break;
+    stage_ready();
+    if (i + 2 < s1) row_a = issue(q_st0, g_st0, stat0);
+#pragma unroll
+    for (int rb = 0; rb < C::NB; ++rb) block(q_st1, g_st1, stat1, rb, row_b);
+  }
+
+  if (it.n_chunks > 1) {  // a part: [wave][dK, dV][d block][register][lane]
+    float* part = A.partial + (it.part * 4 + wave) * (2 * ND * 16 * 64) + lane;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        part[(d * 16 + e) * 64] = dk[d][e];
+        part[((ND + d) * 16 + e) * 64] = dv[d][e];
+      }
+    return;
+  }
+  const bool met = key_in && !(sum_finite(dk) && sum_finite(dv));
+  if (key_in) store_keys<D, E>(A, b, kvh, j, hf, dk, dv);
+  fix_keys<E>(A, si, b, kvh, jw0, sink_end, met, lane);
+}
+
+// The parts of one cut key block, summed in their order.
+template <int D, Elem E>
+__global__ __launch_bounds__(256) void sink_join_kernel(SinkArgs A) {
+  using T = SinkTile<D, E>;
+  constexpr int ND = T::ND;
+  const int n_cut = A.chunks > 1 ? A.nkb : A.n_sink_blocks;
+  const int bkv = blockIdx.x / n_cut, kblk = blockIdx.x - bkv * n_cut;
+  const bool sink = kblk < A.n_sink_blocks;
+  const int n = sink ? A.sink_chunks : A.chunks;
+  if (n == 1) return;
+  const int units = A.n_sink_blocks * A.sink_chunks + (A.nkb - A.n_sink_blocks) * A.chunks;
+  const int u = sink ? kblk * A.sink_chunks
+                     : A.n_sink_blocks * A.sink_chunks + (kblk - A.n_sink_blocks) * A.chunks;
+  const KeyItem it = key_item(A, bkv * units + u);
+  const SeqInfo si = seq_info(A, it.b);
+  const int sink_end = min(si.first + A.sinks, A.kv_len);
+  const int tid = threadIdx.x;
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int jw0 = si.first + kblk * 128 + wave * 32;
+  if (jw0 >= A.kv_len) return;
+  const int j = jw0 + (lane & 31);
+  f32x16 dk[ND], dv[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
+  for (int c = 0; c < n; ++c) {
+    const float* part = A.partial + ((it.part + c) * 4 + wave) * (2 * ND * 16 * 64) + lane;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        dk[d][e] += part[(d * 16 + e) * 64];
+        dv[d][e] += part[((ND + d) * 16 + e) * 64];
+      }
+  }
+  const bool key_in = j < A.kv_len;
+  const bool met = key_in && !(sum_finite(dk) && sum_finite(dv));
+  if (key_in) store_keys<D, E>(A, it.b, it.kvh, j, lane >> 5, dk, dv);
+  fix_keys<E>(A, si, it.b, it.kvh, jw0, sink_end, met, lane);
+}
+
+template <int D, Elem E>
+hipError_t launch_bwd(const SinkArgs& a, hipStream_t stream) {
+  const int64_t rows = (int64_t)a.B * a.H * a.q_len;
+  sink_prep_kernel<E><<<(unsigned)std::min<int64_t>((rows + 15) / 16, 1 << 20), 256, 0, stream>>>(a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  SinkArgs g = a;
+  const int64_t n_dq = (int64_t)a.B * a.H * a.nqb;
+  g.xcd_runs = sink_xcd_runs(a, n_dq);
+  sink_dq_kernel<D, E><<<(unsigned)n_dq, 256, 0, stream>>>(g);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int64_t units = (int64_t)a.n_sink_blocks * a.sink_chunks +
+                        (int64_t)(a.nkb - a.n_sink_blocks) * a.chunks;
+  const int64_t n_kv = (int64_t)a.B * a.Hkv * units;
+  g.xcd_runs = sink_xcd_runs(a, n_kv);
+  sink_dkdv_kernel<D, E><<<(unsigned)n_kv, 256, 0, stream>>>(g);
+  e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int64_t n_cut = a.chunks > 1 ? a.nkb : a.n_sink_blocks;
+  if (n_cut > 0 && (a.chunks > 1 || a.sink_chunks > 1)) {
+    sink_join_kernel<D, E><<<(unsigned)(a.B * a.Hkv * n_cut), 256, 0, stream>>>(g);
+    e = hipGetLastError();
+  }
+  return e;
+}
+
+template <Elem E>
+hipError_t launch_elem(const SinkArgs& a, hipStream_t stream) {
+  return a.d_real <= 64 ? launch_bwd<64, E>(a, stream) : launch_bwd<128, E>(a, stream);
+}
+
+}  // namespace
+
+hipError_t launch_sink_bwd(const SinkArgs& a, hipStream_t stream) {
+  (void)hipGetLastError();
+  if (a.elem == (int)Elem::f32) return launch_elem<Elem::f32>(a, stream);
+  if (a.elem == (int)Elem::bf16) return launch_elem<Elem::bf16>(a, stream);
+  return launch_elem<Elem::f16>(a, stream);
+}
+
+}  // namespace esa

@@ -1155,12 +1155,17 @@ class ElasticSparseAttention(nn.Module):
     Args mirror :375-386.  ``scaling = head_dim ** -0.5`` (:444),
     ``num_kv_groups = H // Hkv`` (:442); query head h reads kv head
     ``h // num_kv_groups`` (:89).
+
+    ``rotary`` (no reference counterpart): a :class:`qk_norm_rope.QKNormRope`
+    that norms and rotates queries and keys before the attention; forward then
+    takes the rows as the projections leave them, and with ``kv_cache`` the
+    new rows of sequences that keep caches.
     """
 
     def __init__(self, layer_idx: int, num_hidden_layers: int, num_attention_heads: int,
                  head_dim: int, attention_length: int, max_seq_len: int,
                  num_key_value_heads: Optional[int] = None, attention_dropout: float = 0.0,
-                 implementation: str = "triton"):
+                 implementation: str = "triton", rotary: Optional[nn.Module] = None):
         super().__init__()
         valid_implementations = ["triton", "naive", "dense"]
         if implementation not in valid_implementations:                   # :412-417
@@ -1183,6 +1188,7 @@ class ElasticSparseAttention(nn.Module):
                 f"`num_key_value_heads` ({self.num_key_value_heads}) for GQA.")
         self.num_kv_groups = self.num_attention_heads // self.num_key_value_heads  # :442
         self.scaling = self.head_dim ** -0.5                                  # :444
+        self.rotary = rotary
         self.pattern = make_pattern(max_seq_len, attention_length, layer_idx,
                                     num_hidden_layers, num_attention_heads)
         self._layouts: Dict[torch.device, ElasticLayout] = {}
@@ -1317,10 +1323,34 @@ class ElasticSparseAttention(nn.Module):
             raise IndexError(f"cache_position out of range for kv_len {kv_len}")
         return pos.to(device)
 
+    def _prepared(self, q, k, v, cache_position, kv_cache):
+        """q and the keys and values to attend over, through ``rotary``; with
+        ``kv_cache`` the checks of the call come before the caches are
+        written."""
+        if self.rotary is None:
+            raise ValueError("kv_cache needs a layer with `rotary`")
+        _check_qkv(q, k, v)
+        if q.shape[1] != self.num_attention_heads or k.shape[1] != self.num_key_value_heads:
+            raise ValueError(
+                f"expected {self.num_attention_heads} query heads and "
+                f"{self.num_key_value_heads} key/value heads; got {q.shape[1]} and {k.shape[1]}")
+        if kv_cache is not None:
+            kv_len = kv_cache[0].shape[2]
+            if kv_len > self.max_seq_len:
+                raise ValueError(
+                    f"Input sequence length ({kv_len}) exceeds the maximum length initialized "
+                    f"in the module ({self.max_seq_len}).")
+            if isinstance(cache_position, torch.Tensor) and cache_position.dim() > 1:
+                raise ValueError("cache_position must be [q_len], shared by the batch")
+        return self.rotary.attention_rows(q, k, v, cache_position, kv_cache)
+
     def forward(self, query_states: torch.Tensor, key_states: torch.Tensor,
-                value_states: torch.Tensor, cache_position: Optional[torch.LongTensor] = None
+                value_states: torch.Tensor, cache_position: Optional[torch.LongTensor] = None,
+                kv_cache: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
                 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
         q, k, v = query_states, key_states, value_states
+        if self.rotary is not None or kv_cache is not None:
+            q, k, v = self._prepared(q, k, v, cache_position, kv_cache)
         _check_qkv(q, k, v)
         B, H, Lq, D = q.shape
         kv_len = k.shape[2]

@@ -41,6 +41,8 @@ EXPORTED = (
     "esa_elastic_bwd_rows", "esa_reachability",
     "esa_qk_norm_rope_fwd", "esa_qk_norm_rope_append", "esa_qk_norm_rope_bwd_workspace_size",
     "esa_qk_norm_rope_bwd",
+    "esa_sink_window_fwd_workspace_size", "esa_sink_window_fwd",
+    "esa_sink_window_bwd_workspace_size", "esa_sink_window_bwd",
 )
 
 
@@ -104,6 +106,16 @@ class EsaNaiveOpts(ctypes.Structure):
         ("weights", ctypes.c_void_p),
         ("weights_stride_b", ctypes.c_int64), ("weights_stride_h", ctypes.c_int64),
         ("weights_stride_s", ctypes.c_int64),
+    ]
+
+
+class EsaWindow(ctypes.Structure):
+    _fields_ = [
+        ("window", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+        ("positions", ctypes.c_void_p),
+        ("position_stride_b", ctypes.c_int64),
+        ("first_key", ctypes.c_void_p),
     ]
 
 
@@ -222,6 +234,15 @@ def load() -> ctypes.CDLL:
     lib.esa_qk_norm_rope_bwd_workspace_size.argtypes = [P(EsaRotaryArgs), P(ctypes.c_size_t)]
     lib.esa_qk_norm_rope_bwd.restype = st
     lib.esa_qk_norm_rope_bwd.argtypes = [P(EsaRotaryArgs), vp, ctypes.c_size_t, vp]
+    size = P(ctypes.c_size_t)
+    lib.esa_sink_window_fwd_workspace_size.restype = st
+    lib.esa_sink_window_fwd_workspace_size.argtypes = [P(EsaFwdArgs), P(EsaWindow), size]
+    lib.esa_sink_window_fwd.restype = st
+    lib.esa_sink_window_fwd.argtypes = [P(EsaFwdArgs), P(EsaWindow), vp, ctypes.c_size_t, vp]
+    lib.esa_sink_window_bwd_workspace_size.restype = st
+    lib.esa_sink_window_bwd_workspace_size.argtypes = [P(EsaBwdArgs), P(EsaWindow), size]
+    lib.esa_sink_window_bwd.restype = st
+    lib.esa_sink_window_bwd.argtypes = [P(EsaBwdArgs), P(EsaWindow), vp, ctypes.c_size_t, vp]
     _lib = lib
     return lib
 

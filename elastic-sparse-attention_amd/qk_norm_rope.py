@@ -333,6 +333,7 @@ class QKNormRope(nn.Module):
         half = rotary_dim // 2
         inv_freq = base ** (-torch.arange(half, dtype=torch.float64) / half)
         self.register_buffer("inv_freq", inv_freq, persistent=False)
+        self._arange: Optional[torch.Tensor] = None  # positions of whole sequences
 
     def _apply(self, fn, *args, **kwargs):
         # the frequencies stay float64 under .half(), .bfloat16() and .to(dtype):
@@ -367,6 +368,26 @@ class QKNormRope(nn.Module):
                              "torch.no_grad(), or use forward")
         return qk_norm_rope_append(q, k, v, k_cache, v_cache, self.q_weight, self.k_weight,
                                    self.inv_freq, cache_position, self.eps, self.interleaved)
+
+    def attention_rows(self, q, k, v, cache_position, kv_cache):
+        """What an attention layer with this module as its ``rotary`` attends
+        over: q and k normed and rotated at their rows' places or, with
+        ``kv_cache`` (the pair of caches), q and the caches after
+        :meth:`append`."""
+        if kv_cache is None:
+            if cache_position is not None:
+                raise ValueError("a layer with `rotary` takes cache_position together with "
+                                 "kv_cache: its k and v are the new rows")
+            n = q.shape[2]
+            if self._arange is None or self._arange.numel() != n or \
+                    self._arange.device != q.device:
+                self._arange = torch.arange(n, device=q.device)
+            q, k = self(q, k, self._arange)
+            return q, k, v
+        if cache_position is None:
+            raise ValueError("kv_cache needs cache_position")
+        k_cache, v_cache = kv_cache
+        return self.append(q, k, v, k_cache, v_cache, cache_position), k_cache, v_cache
 
     def _check_dim(self, q: torch.Tensor) -> None:
         if q.dim() != 4 or q.shape[-1] != self.head_dim:

@@ -574,6 +574,51 @@ esa_status esa_qk_norm_rope_bwd_workspace_size(const esa_rotary_args* a, size_t*
 esa_status esa_qk_norm_rope_bwd(const esa_rotary_args* a, void* workspace,
                                 size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Attention over a causal sliding window and a few first keys that stay
+ * visible (sinks).  No reference counterpart: the reference's own window is
+ * its layer 0, attention_length keys and no others.
+ *
+ * Row r of sequence b sits at position p; it sees key j when
+ *   f <= j <= p  and  (p - j < window  or  j - f < sinks).
+ * f is the sequence's first key (left padding), 0 without first_key; one
+ * outside [0, kv_len] is taken as the nearer end.  A row before f sees nothing:
+ * o = 0, lse = -inf, no gradient.  Whatever a hidden key or row holds (Inf and
+ * NaN too) reaches nothing.
+ *
+ * positions: row r of a sequence sits at its first position (a negative one
+ * counting from kv_len) + r; a row whose own entry says otherwise, or that
+ * lies outside the cache, gets o = NaN.  Without positions row r is position
+ * r, and q_len <= kv_len. */
+typedef struct esa_window {
+  int32_t window; /* >= 1 */
+  int32_t sinks;  /* >= 0 */
+  const int64_t* positions;  /* device, [q_len] a sequence, or NULL */
+  int64_t position_stride_b; /* 0: shared by the batch */
+  const int64_t* first_key;  /* device, [batch], or NULL */
+} esa_window;
+
+/* Host only.  Workspace of esa_sink_window_fwd: 0 but for a few rows against
+ * many keys, whose key ranges are computed side by side and joined. */
+esa_status esa_sink_window_fwd_workspace_size(const esa_fwd_args* a, const esa_window* w,
+                                              size_t* bytes);
+
+/* o and (where given) lse of q, k, v: any q_len, so decode steps, chunks at
+ * their positions and whole sequences.  head_dim: a multiple of 8 (float32: of
+ * 4) up to 128; pointers 16-byte aligned, strides in whole 16 bytes, the row
+ * strides of k and v below 16 MiB. */
+esa_status esa_sink_window_fwd(const esa_fwd_args* a, const esa_window* w, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* Host only.  Workspace of esa_sink_window_bwd. */
+esa_status esa_sink_window_bwd_workspace_size(const esa_bwd_args* a, const esa_window* w,
+                                              size_t* bytes);
+
+/* dq, dk, dv from the forward's inputs, o, lse and the gradient of o; every
+ * element of the three is written, sums in a fixed order (no atomics). */
+esa_status esa_sink_window_bwd(const esa_bwd_args* a, const esa_window* w, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
