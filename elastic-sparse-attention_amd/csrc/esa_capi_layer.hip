@@ -232,21 +232,73 @@ esa_status sink_fwd_shape(const esa_fwd_args* a, const esa_window* w) {
 // Row stride of delta and lse2 (whole 16 bytes a head)
 int sink_qpad(int q_len) { return (q_len + 3) / 4 * 4; }
 
-// How the rows of a key block are cut.  A block is walked by one workgroup
-// while the grid fills the chip; a sinks' block, which every later row sees, is
-// cut into pieces of about a window block's rows.
+// How the rows of a kv head's key blocks are cut, in stages of 64 rows and
+// heads.  The chip runs `slots` blocks at a time; a chunk costs what its stages
+// do and about `part` stages more for its float32 part (written, read and
+// joined).  Counted so, with the blocks alike (a window):
+//   a sinks' block is cut into pieces of a window block's size;
+//   of U blocks the whole rounds stay whole, and the U mod slots that would
+//   fill a last round by themselves are cut so that they fill it together
+//   (8192 rows, 8 kv heads of 4 query heads, window 1024, head_dim 128: 568
+//   blocks on 512 slots, two rounds of 76 stages against one and a ninth);
+// where the first blocks see many more rows than the last (a window near the
+// sequence's length) all are cut alike, to at most 2/3 of a slot's share.
 void sink_bwd_plan(SinkArgs& g) {
   g.nkb = (g.kv_len + 127) / 128;
-  g.n_sink_blocks = std::min(g.nkb, (g.sinks + 127) / 128);
   g.qpad = sink_qpad(g.q_len);
-  const int64_t blocks = (int64_t)g.B * g.Hkv * g.nkb;
-  const int64_t rows = std::min<int64_t>(g.q_len, (int64_t)g.window + 127);  // a block's, at most
-  const int64_t stages = (rows + 63) / 64 * g.groups;
-  g.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(stages / 4, 512 / blocks));
-  const int64_t ratio = ((int64_t)g.q_len + rows - 1) / rows;
-  const int64_t sink_blocks = std::max<int64_t>(1, (int64_t)g.B * g.Hkv * g.n_sink_blocks);
-  g.sink_chunks = (int)std::min<int64_t>(std::min<int64_t>(64, ratio * g.chunks),
-                                         std::max<int64_t>(1, 2048 / sink_blocks));
+  const int64_t slots = g.elem == ESA_F32 ? 256 : 512, part = 6;
+  const int64_t kv = (int64_t)g.B * g.Hkv;
+  const int n_sink = std::min(g.nkb, (g.sinks + 127) / 128);
+  auto stages = [&](int64_t rows) { return (rows + 63) / 64 * g.groups; };
+  const int64_t one = stages(std::min<int64_t>(g.q_len, (int64_t)g.window + 127));
+  // a block's rows are cut short by the sequence's end: the average of them
+  const int64_t n_reg = g.nkb - n_sink;
+  const int64_t span = std::min<int64_t>(g.window + 127, g.q_len);
+  const double mean = 1.0 - 0.5 * (double)span / (double)std::max<int64_t>(g.q_len, 1);
+  int cut[2] = {1, 1};
+  int64_t n_last = 0;
+  auto best_cut = [&](int64_t blocks, int64_t whole_rounds) {
+    int64_t best = 0;
+    int c_best = 1;
+    for (int c = 1; c <= 16 && c <= one; ++c) {
+      const int64_t rounds = (blocks * c + slots - 1) / slots;
+      const int64_t cost = whole_rounds * one + rounds * ((one + c - 1) / c + (c > 1 ? part : 0));
+      if (c == 1 || cost < best) {
+        best = cost;
+        c_best = c;
+      }
+    }
+    return c_best;
+  };
+  if (n_reg > 0) {
+    if (mean < 0.75) {
+      const double share = (double)kv * n_reg * one * mean / (double)slots;
+      cut[0] = cut[1] = (int)std::max(1.0, std::min(8.0, std::ceil(1.5 * one / share)));
+      cut[0] = cut[1] = (int)std::max<int64_t>(1, std::min<int64_t>(cut[0], 4 * slots / (kv * n_reg)));
+    } else {
+      const int64_t blocks = kv * n_reg, over = blocks % slots;
+      if (blocks < slots) {
+        cut[0] = cut[1] = best_cut(blocks, 0);
+      } else if (over > 0 && blocks < 8 * slots) {
+        cut[1] = best_cut(over, blocks / slots);
+        n_last = cut[1] > 1 ? (over + kv - 1) / kv : 0;
+      }
+    }
+  }
+  // the sinks' pieces as long as the shortest chunk of the others, within
+  // 256 MiB of parts
+  int64_t sink_cut = 1;
+  if (n_sink > 0) {
+    const int64_t piece = std::max<int64_t>(1, one / std::max(1, cut[0]));
+    sink_cut = std::min<int64_t>(64, (stages(g.q_len) + piece - 1) / piece);
+    sink_cut = std::min(sink_cut, std::max<int64_t>(1, 2048 / (kv * n_sink)));
+  }
+  g.cls_n[0] = n_sink;
+  g.cls_cut[0] = (int)sink_cut;
+  g.cls_n[2] = (int)std::min<int64_t>(n_last, n_reg);
+  g.cls_n[1] = (int)n_reg - g.cls_n[2];
+  g.cls_cut[1] = cut[0];
+  g.cls_cut[2] = cut[1];
 }
 
 struct SinkBwdSizes {
@@ -256,8 +308,8 @@ struct SinkBwdSizes {
 SinkBwdSizes sink_bwd_sizes(const SinkArgs& g) {
   SinkBwdSizes z;
   z.stat = ((size_t)g.B * g.H * g.qpad * sizeof(float) + 255) / 256 * 256;
-  const size_t cut = (g.sink_chunks > 1 || g.chunks > 1 ? (size_t)g.n_sink_blocks * g.sink_chunks : 0) +
-                     (g.chunks > 1 ? (size_t)(g.nkb - g.n_sink_blocks) * g.chunks : 0);
+  size_t cut = 0;
+  for (int c = 0; c < 3; ++c) cut += g.cls_cut[c] > 1 ? (size_t)g.cls_n[c] * g.cls_cut[c] : 0;
   z.part = (size_t)g.B * g.Hkv * cut * 2 * 128 * (g.d_real <= 64 ? 64 : 128) * sizeof(float);
   return z;
 }

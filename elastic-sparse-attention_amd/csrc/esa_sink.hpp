@@ -33,9 +33,12 @@ struct SinkArgs {
   float* delta;  // [B, H, qpad] rowsum(dO * O)
   float* lse2;   // [B, H, qpad] log2(e) * lse
   int qpad;
-  int nkb, n_sink_blocks;     // 128-key blocks a kv head; the first ones hold sinks
-  int chunks, sink_chunks;    // row chunks of a block, of a sink block
-  float* partial;             // partial sums of blocks with more than one chunk
+  // a kv head's 128-key blocks in three classes, one after the other (the
+  // sinks', the next, the last): their numbers and how many chunks the rows
+  // of each class' blocks are cut into
+  int nkb;
+  int cls_n[3], cls_cut[3];
+  float* partial;             // partial sums of the blocks with more than one chunk
   // decode
   int splits;                 // key ranges a (sequence, kv head, row tile)
   int row_tiles;              // 16-row tiles of its groups * q_len rows
@@ -122,6 +125,32 @@ struct KeyStages {
     return i < n_sink ? f + i * step : m0 + (i - n_sink) * step;
   }
 };
+// What the rows [p0, p0 + 31] of one wave (its last one p1, no row: p1 < p0)
+// see of those stages, as ranges of their indices: none of a stage past `last`,
+// or before `first` and the sinks; every pair of stages full_lo .. full_hi.
+// (Sink stages count as partly seen.)
+struct WaveStages {
+  int last, first, sinks, full_lo, full_n;
+  __device__ __forceinline__ bool sees(int i) const {
+    return i <= last && (i >= first || i < sinks);
+  }
+  __device__ __forceinline__ bool full(int i) const { return (uint32_t)(i - full_lo) < (uint32_t)full_n; }
+};
+template <int STAGE>
+__device__ __forceinline__ WaveStages wave_stages(const KeyStages& k, int p0, int p1, int window,
+                                                  int sink_end) {
+  auto floor_div = [](int a) { return a >> (STAGE == 64 ? 6 : 5); };
+  static_assert(STAGE == 64 || STAGE == 32, "stage");
+  WaveStages w;
+  // k0 <= p1;  k0 + STAGE - 1 > p0 - window;  k0 < sink_end
+  w.last = p1 < p0 ? -1 : k.n_sink + max(floor_div(p1 - k.m0), -1);
+  w.first = k.n_sink + floor_div(max(p0 - window + 1 - k.m0, 0));
+  w.sinks = k.n_sink + (sink_end > k.m0 ? floor_div(sink_end - 1 - k.m0) + 1 : 0);
+  // k0 > p0 + 31 - window and k0 + STAGE - 1 <= p0
+  w.full_lo = k.n_sink + max(floor_div(p0 + 31 - window - k.m0) + 1, 0);
+  w.full_n = max(k.n_sink + floor_div(p0 + 1 - k.m0) - w.full_lo, 0);
+  return w;
+}
 template <int STAGE>
 __device__ __forceinline__ KeyStages key_stages(const SinkArgs& A, const SeqInfo& si, int r0,
                                                 int sink_end) {
@@ -150,7 +179,10 @@ __device__ __forceinline__ KeyStages key_stages(const SinkArgs& A, const SeqInfo
 // Accumulator register r of lane half hf is row 8 (r / 4) + 4 hf + r % 4.
 // LDS rows are D elements unpadded, their 16-byte chunks XOR-swizzled by the
 // row, so that both kinds of read meet each bank once.
-template <int D, Elem E>
+// TIGHT: a kernel short of registers forms a read's address from one base with
+// an exclusive or (the chunk's bits, which the swizzle and the read's place
+// share) each time, instead of keeping one register a read.
+template <int D, Elem E, bool TIGHT = false>
 struct SinkTile {
   using M = MmaT<E>;
   using V8 = typename M::v8;
@@ -167,8 +199,8 @@ struct SinkTile {
   using LdsT = uint16_t;
   static constexpr uint32_t kOne = E == Elem::bf16 ? 0x3F80u : 0x3C00u;
 
-  int ra[NS];  // element offsets of a 32-row block's row reads
-  int ca[ND];  // ... of its column reads, rows 4 hf + 0 .. 3 (+ 16 u)
+  int ra[TIGHT ? 1 : NS];  // element offsets of a 32-row block's row reads
+  int ca[TIGHT ? 1 : ND];  // ... of its column reads, rows 4 hf + 0 .. 3 (+ 16 u)
   int hf;
 
   static __device__ __forceinline__ int swz(int row) { return swz_k<(D >= 128 ? 128 : 64)>(row); }
@@ -176,10 +208,10 @@ struct SinkTile {
     hf = lane >> 5;
     const int l32 = lane & 31, g4 = lane >> 4, lam = lane & 15;
 #pragma unroll
-    for (int s = 0; s < NS; ++s) ra[s] = l32 * D + 8 * ((2 * s + hf) ^ swz(l32));
+    for (int s = 0; s < (TIGHT ? 1 : NS); ++s) ra[s] = l32 * D + 8 * ((2 * s + hf) ^ swz(l32));
     const int row = 4 * hf + (lam >> 2);
 #pragma unroll
-    for (int d = 0; d < ND; ++d) {
+    for (int d = 0; d < (TIGHT ? 1 : ND); ++d) {
       const int col = 32 * d + 16 * (g4 & 1) + 4 * (lam & 3);
       ca[d] = row * D + 8 * ((col >> 3) ^ swz(row)) + (col & 7);
     }
@@ -197,9 +229,24 @@ struct SinkTile {
                                               const Frag& f) const {
     V8 a[NS];
 #pragma unroll
-    for (int s = 0; s < NS; ++s) a[s] = *(const V8*)(buf + ra[s] + 32 * rb * D);
+    for (int s = 0; s < NS; ++s) a[s] = row_operand(buf, rb, s);
 #pragma unroll
     for (int s = 0; s < NS; ++s) acc = M::mfma32(a[s], f.f[s], acc);
+  }
+  // element offset `x` of a base, formed where it is used (the empty asm keeps
+  // the compiler from forming all of them ahead and keeping them)
+  static __device__ __forceinline__ int offset(int base, int x) {
+    if constexpr (TIGHT) asm volatile("" : "+v"(base));
+    return base ^ x;
+  }
+  __device__ __forceinline__ V8 row_operand(const LdsT* buf, int rb, int s) const {
+    const int at = TIGHT ? offset(ra[0], 16 * s) : ra[s];
+    return *(const V8*)(buf + at + 32 * rb * D);
+  }
+  // one product of col_product: rows 16 u .. of the block
+  static __device__ __forceinline__ void col_step(f32x16& acc, const u32x4& a, const P& p, int u) {
+    const u32x4 b = {p.w[4 * u], p.w[4 * u + 1], p.w[4 * u + 2], p.w[4 * u + 3]};
+    acc = M::mfma32(__builtin_bit_cast(V8, a), __builtin_bit_cast(V8, b), acc);
   }
   __device__ __forceinline__ P pack(const f32x16& v) const {
     P p;
@@ -209,8 +256,9 @@ struct SinkTile {
   }
   // the A operand of dims 32 d .. and rows 16 u .. of block rb, by columns
   __device__ __forceinline__ u32x4 col_operand(const LdsT* buf, int rb, int d, int u) const {
-    const LdsT* p1 = buf + ca[d] + (32 * rb + 16 * u) * D;
-    const LdsT* p2 = buf + (ca[d] ^ 16) + (32 * rb + 16 * u + 8) * D;
+    const int at = TIGHT ? offset(ca[0], 32 * d) : ca[d];
+    const LdsT* p1 = buf + at + (32 * rb + 16 * u) * D;
+    const LdsT* p2 = buf + (at ^ 16) + (32 * rb + 16 * u + 8) * D;
     const s16x4 v[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p1),
                         __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p2)};
     return __builtin_bit_cast(u32x4, v);
@@ -243,8 +291,8 @@ struct SinkTile {
   }
 };
 
-template <int D>
-struct SinkTile<D, Elem::f32> {
+template <int D, bool TIGHT>
+struct SinkTile<D, Elem::f32, TIGHT> {
   static constexpr int ES = 4;
   static constexpr int EPC = 4;
   static constexpr int NU = D / 8, ND = D / 32;
@@ -315,10 +363,13 @@ struct SinkTile<D, Elem::f32> {
   }
 };
 
-// ROWS rows of D elements from one matrix into LDS, 16 bytes a lane and load:
-// the buffer resource starts at the stage's first row (so a row's offset stays
-// small however long the tensor is) and ends with the last row; whatever lies
-// past it, or past head_dim, reads as zero.
+// ROWS rows of D elements from one matrix into LDS, 16 bytes a lane and load.
+// The buffer resource starts at a row of the matrix (`org`) and ends with its
+// last one; a stage is reached by the scalar offset of its first row, and past
+// 1 GiB from org the resource moves on, so offsets stay small however long the
+// tensor is.  Whatever lies past the last row, or past head_dim, reads as zero.
+// (A resource formed anew for every stage cost more scalar instructions than
+// the stage's products have vector ones, and a third of the forward's time.)
 template <int D, Elem E, int ROWS, int THREADS>
 struct SinkStage {
   using T = SinkTile<D, E>;
@@ -326,10 +377,12 @@ struct SinkStage {
   static constexpr int BYTES = ROWS * D * T::ES;
   static_assert(LOADS >= 1 && LOADS * THREADS == ROWS * T::CPR, "whole stage per load round");
   int off[LOADS];
+  __amdgpu_buffer_rsrc_t rs;
   const char* base;
   int64_t stride;  // bytes
   int rows;        // rows of the matrix
   int row_bytes;
+  int org, reach;  // the resource's first row, and how many rows it serves
 
   __device__ __forceinline__ void init(const void* p, int64_t stride_elems, int n_rows, int d_real,
                                        int tid) {
@@ -337,6 +390,8 @@ struct SinkStage {
     stride = stride_elems * T::ES;
     rows = n_rows;
     row_bytes = d_real * T::ES;
+    org = 0;
+    reach = 0;
     const int lane = tid & 63, wave = tid >> 6;
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
@@ -344,16 +399,29 @@ struct SinkStage {
       const int row = slot / T::CPR, chunk = (slot % T::CPR) ^ T::swz(row);
       off[j] = 16 * chunk < row_bytes ? (int)(row * stride) + 16 * chunk : 0x7ffffff0;
     }
+    // (0x7ffffff0 plus a stage's offset, below 2^30, is past every resource as
+    // an unsigned number)
   }
-  // rows row0 .. row0 + ROWS - 1 -> dst
-  __device__ __forceinline__ void issue(int row0, void* dst, int wave) const {
+  // another matrix of the same shape
+  __device__ __forceinline__ void rebase(const void* p) {
+    base = (const char*)p;
+    reach = 0;
+  }
+  __device__ __forceinline__ void move(int row0) {
     const int64_t left = (int64_t)(rows - row0 - 1) * stride + row_bytes;
     const int n = rows > row0 ? (int)(left < 0x7fffff00 ? left : 0x7fffff00) : 0;
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-        (void*)(base + (int64_t)row0 * stride), (short)0, n, 0x00020000);
+    rs = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)row0 * stride), (short)0, n,
+                                           0x00020000);
+    org = row0;
+    reach = (int)((1u << 30) / (uint32_t)(stride > 16 ? stride : 16));
+  }
+  // rows row0 .. row0 + ROWS - 1 -> dst
+  __device__ __forceinline__ void issue(int row0, void* dst, int wave) {
+    if ((uint32_t)(row0 - org) >= (uint32_t)reach) move(row0);
+    const int soff = (row0 - org) * (int)stride;
 #pragma unroll
     for (int j = 0; j < LOADS; ++j)
-      load_lds16(rs, (uint16_t*)dst + (LOADS * wave + j) * 512, off[j], 0);
+      load_lds16(rs, (uint16_t*)dst + (LOADS * wave + j) * 512, off[j], soff);
   }
 };
 
@@ -362,6 +430,14 @@ struct SinkStage {
 __device__ __forceinline__ void stage_ready() {
   __builtin_amdgcn_s_waitcnt(kWaitVmcnt0);
   __syncthreads();
+}
+
+// Waits until at most LATER of this wave's loads are on their way, then for
+// the other waves.
+template <int LATER>
+__device__ __forceinline__ void stage_wait() {
+  static_assert(LATER < 64, "vmcnt counts to 63");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
 }
 
 // Non-finite values.  A staged block also holds rows that a column does not

@@ -15,10 +15,10 @@
 //   sink_join_kernel  blocks whose rows were split: the parts in order
 //
 // Key blocks start at the sequence's first key, so the sinks are in the first
-// ones.  A sink is seen by every later row: its block's rows (all query heads
-// of the kv group, one after the other) are cut into `sink_chunks` workgroups
-// of about a window block's rows each, which leave float32 parts; other blocks
-// are cut into `chunks` where the grid alone would not fill the chip.
+// ones.  A block's rows are those of every query head of the kv group, one
+// after the other, and may be cut into chunks, one workgroup each, that leave
+// float32 parts: a sink's block, which every later row sees, and the blocks
+// that would run as an unfilled last round of the grid (sink_bwd_plan).
 #include <algorithm>
 
 #include "esa_sink.hpp"
@@ -223,29 +223,48 @@ struct KeyItem {
   int b, kvh, kblk, chunk, n_chunks;
   int64_t part;  // index of its float32 part
 };
-__device__ __forceinline__ KeyItem key_item(const SinkArgs& A, int item) {
-  const int n_reg = A.nkb - A.n_sink_blocks;
-  const int units = A.n_sink_blocks * A.sink_chunks + n_reg * A.chunks;
-  const int bkv = item / units;
-  int u = item - bkv * units;
+// parts a kv head keeps
+__device__ __host__ __forceinline__ int kv_parts(const SinkArgs& A) {
+  int n = 0;
+  for (int c = 0; c < 3; ++c) n += A.cls_cut[c] > 1 ? A.cls_n[c] * A.cls_cut[c] : 0;
+  return n;
+}
+// Block `block` of class `cls` of kv head bkv (over the batch), one chunk of it
+__device__ __forceinline__ KeyItem key_block(const SinkArgs& A, int bkv, int cls, int block,
+                                             int chunk) {
   KeyItem k;
   k.b = bkv / A.Hkv;
   k.kvh = bkv - k.b * A.Hkv;
-  const int n_sink_units = A.n_sink_blocks * A.sink_chunks;
-  if (u < n_sink_units) {
-    k.kblk = u / A.sink_chunks;
-    k.chunk = u - k.kblk * A.sink_chunks;
-    k.n_chunks = A.sink_chunks;
-  } else {
-    const int w = u - n_sink_units;
-    k.kblk = w / A.chunks;
-    k.chunk = w - k.kblk * A.chunks;
-    k.n_chunks = A.chunks;
-    k.kblk += A.n_sink_blocks;
+  k.kblk = block;
+  k.chunk = chunk;
+  k.n_chunks = A.cls_cut[cls];
+  int at = block * k.n_chunks + chunk;
+  for (int c = 0; c < cls; ++c) {
+    k.kblk += A.cls_n[c];
+    at += A.cls_cut[c] > 1 ? A.cls_n[c] * A.cls_cut[c] : 0;
   }
-  k.part = (int64_t)bkv * (A.n_sink_blocks * A.sink_chunks + (A.chunks > 1 ? n_reg * A.chunks : 0)) +
-           u;
+  k.part = (int64_t)bkv * kv_parts(A) + at;
   return k;
+}
+// The grid's order: class by class (the longest work first), the kv heads of
+// an XCD's run (or all of them) in each class one after the other.
+__device__ __forceinline__ KeyItem key_item(const SinkArgs& A) {
+  int item = blockIdx.x, n_kv = A.B * A.Hkv, kv0 = 0;
+  if (A.xcd_runs) {
+    n_kv >>= 3;
+    kv0 = (item & 7) * n_kv;
+    item >>= 3;
+  }
+  int cls = 0;
+  for (; cls < 2; ++cls) {
+    const int n = n_kv * A.cls_n[cls] * A.cls_cut[cls];
+    if (item < n) break;
+    item -= n;
+  }
+  const int per = A.cls_n[cls] * A.cls_cut[cls];
+  const int kv = item / per, u = item - kv * per;
+  const int block = u / A.cls_cut[cls];
+  return key_block(A, kv0 + kv, cls, block, u - block * A.cls_cut[cls]);
 }
 
 // Stores 32 keys' dK^T and dV^T (one wave's accumulators)
@@ -341,7 +360,7 @@ template <int D, Elem E>
 __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_dkdv_kernel(
     SinkArgs A) {
   using C = SinkBwdCfg<D, E>;
-  using T = SinkTile<D, E>;
+  using T = SinkTile<D, E, (D >= 128)>;
   using Stage = SinkStage<D, E, C::STAGE, 256>;
   using LdsT = typename T::LdsT;
   constexpr int ND = T::ND;
@@ -352,9 +371,7 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
   __shared__ __attribute__((aligned(256))) float stat0[2 * 64];  // lse2, then delta
   __shared__ __attribute__((aligned(256))) float stat1[2 * 64];
 
-  int item = blockIdx.x;
-  if (A.xcd_runs) item = (item & 7) * ((int)gridDim.x >> 3) + (item >> 3);
-  const KeyItem it = key_item(A, item);
+  const KeyItem it = key_item(A);
   const int b = it.b, kvh = it.kvh;
   const SeqInfo si = seq_info(A, b);
   const int f = si.first, sink_end = min(f + A.sinks, A.kv_len), W = A.window;
@@ -410,12 +427,16 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
   qs.init(nullptr, A.qss, A.q_len, A.d_real, tid);
   gs.init(nullptr, A.doss, A.q_len, A.d_real, tid);
   int head = per_head > 0 ? s0 / per_head : 0, at_stage = s0 - head * per_head;
+  int staged = -1;
   // the next stage in order -> buffers; returns its first row
   auto issue = [&](LdsT* qd, LdsT* gd, float* stat) __attribute__((always_inline)) {
     const int h = kvh * A.groups + head;
     const int row0 = p_lo - si.base + at_stage * C::STAGE;
-    qs.base = (const char*)at<E>(A.q, (int64_t)b * A.qsb + (int64_t)h * A.qsh);
-    gs.base = (const char*)at<E>(A.dout, (int64_t)b * A.dosb + (int64_t)h * A.dosh);
+    if (h != staged) {  // another head's rows
+      qs.rebase(at<E>(A.q, (int64_t)b * A.qsb + (int64_t)h * A.qsh));
+      gs.rebase(at<E>(A.dout, (int64_t)b * A.dosb + (int64_t)h * A.dosh));
+      staged = h;
+    }
     qs.issue(row0, qd, wave);
     gs.issue(row0, gd, wave);
     // lse2 and delta, 64 rows each, zeros past q_len: copied to LDS like the
@@ -441,21 +462,29 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
     f32x16 s = f32x16{}, dp = f32x16{};
     if (p0 + 31 > p_last || !all_seen(p0, p0 + 31, jw0, W, sink_end))
       mask_init<0>(s, ~(seen_rows(j, p0, p_last, W, sink_end) >> (4 * hf)));
+    // (one product's operands at a time: the accumulators, K and V leave room
+    // for no more)
     t.row_product(s, qb, rb, kf);
-    f32x4 l2[4], dl[4];
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      l2[q] = *(const f32x4*)(stat + 32 * rb + 8 * q + 4 * hf);
-      dl[q] = *(const f32x4*)(stat + 64 + 32 * rb + 8 * q + 4 * hf);
+      const f32x4 l2 = *(const f32x4*)(stat + 32 * rb + 8 * q + 4 * hf);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        s[4 * q + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + e], scale, -l2[e]));
     }
     t.row_product(dp, gb, rb, vf);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -l2[i / 4][i % 4]));
-      dp[i] = s[i] * (dp[i] - dl[i / 4][i % 4]);
-    }
+    __builtin_amdgcn_sched_barrier(0);
     t.col_product(dv, gb, rb, t.pack(s));
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 dl = *(const f32x4*)(stat + 64 + 32 * rb + 8 * q + 4 * hf);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dp[4 * q + e] = s[4 * q + e] * (dp[4 * q + e] - dl[e]);
+    }
     t.col_product(dk, qb, rb, t.pack(dp));
+    __builtin_amdgcn_sched_barrier(0);
   };
   int row_a = 0, row_b = 0;
   if (s0 < s1) row_a = issue(q_st0, g_st0, stat0);
@@ -487,44 +516,69 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
   fix_keys<E>(A, si, b, kvh, jw0, sink_end, met, lane);
 }
 
-// The parts of one cut key block, summed in their order.
+// The parts of one cut key block's 32 keys, summed in their order: each wave
+// takes the 32-dim pieces of dK and dV in turn.
 template <int D, Elem E>
 __global__ __launch_bounds__(256) void sink_join_kernel(SinkArgs A) {
   using T = SinkTile<D, E>;
   constexpr int ND = T::ND;
-  const int n_cut = A.chunks > 1 ? A.nkb : A.n_sink_blocks;
-  const int bkv = blockIdx.x / n_cut, kblk = blockIdx.x - bkv * n_cut;
-  const bool sink = kblk < A.n_sink_blocks;
-  const int n = sink ? A.sink_chunks : A.chunks;
-  if (n == 1) return;
-  const int units = A.n_sink_blocks * A.sink_chunks + (A.nkb - A.n_sink_blocks) * A.chunks;
-  const int u = sink ? kblk * A.sink_chunks
-                     : A.n_sink_blocks * A.sink_chunks + (kblk - A.n_sink_blocks) * A.chunks;
-  const KeyItem it = key_item(A, bkv * units + u);
+  __shared__ uint32_t met[4][32];
+  int n_cut = 0;
+  for (int c = 0; c < 3; ++c) n_cut += A.cls_cut[c] > 1 ? A.cls_n[c] : 0;
+  const int quarter = blockIdx.x & 3, bkv = (blockIdx.x >> 2) / n_cut;
+  int block = (blockIdx.x >> 2) - bkv * n_cut, cls = 0;
+  for (; cls < 2; ++cls) {
+    const int n = A.cls_cut[cls] > 1 ? A.cls_n[cls] : 0;
+    if (block < n) break;
+    block -= n;
+  }
+  const KeyItem it = key_block(A, bkv, cls, block, 0);
+  const int n = it.n_chunks;
   const SeqInfo si = seq_info(A, it.b);
   const int sink_end = min(si.first + A.sinks, A.kv_len);
   const int tid = threadIdx.x;
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int jw0 = si.first + kblk * 128 + wave * 32;
-  if (jw0 >= A.kv_len) return;
-  const int j = jw0 + (lane & 31);
-  f32x16 dk[ND], dv[ND];
-#pragma unroll
-  for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
-  for (int c = 0; c < n; ++c) {
-    const float* part = A.partial + ((it.part + c) * 4 + wave) * (2 * ND * 16 * 64) + lane;
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        dk[d][e] += part[(d * 16 + e) * 64];
-        dv[d][e] += part[((ND + d) * 16 + e) * 64];
-      }
-  }
+  const int l32 = lane & 31, hf = lane >> 5;
+  const int jw0 = si.first + it.kblk * 128 + quarter * 32;
+  if (jw0 >= A.kv_len) return;  // (the whole workgroup)
+  const int j = jw0 + l32;
   const bool key_in = j < A.kv_len;
-  const bool met = key_in && !(sum_finite(dk) && sum_finite(dv));
-  if (key_in) store_keys<D, E>(A, it.b, it.kvh, j, lane >> 5, dk, dv);
-  fix_keys<E>(A, si, it.b, it.kvh, jw0, sink_end, met, lane);
+  bool bad = false;
+  for (int w = wave; w < 2 * ND; w += 4) {  // dK's pieces, then dV's
+    f32x16 x = f32x16{};
+    const float* part = A.partial + (it.part * 4 + quarter) * (2 * ND * 16 * 64) +
+                        w * (16 * 64) + lane;
+    for (int c = 0; c < n; ++c, part += 4 * 2 * ND * 16 * 64)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) x[e] += part[e * 64];
+    float sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sum += x[e];
+    bad |= !__builtin_isfinite(sum);
+    const bool is_k = w < ND;
+    const int d = is_k ? w : w - ND;
+    const float scale = is_k ? A.sm_scale : 1.f;
+    auto* row = is_k ? (typename ElemT<E>::T*)A.dk + (int64_t)it.b * A.dksb +
+                           (int64_t)it.kvh * A.dksh + (int64_t)j * A.dkss
+                     : (typename ElemT<E>::T*)A.dv + (int64_t)it.b * A.dvsb +
+                           (int64_t)it.kvh * A.dvsh + (int64_t)j * A.dvss;
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      const int dim = 32 * d + 8 * q4 + 4 * hf;
+      if (key_in && dim < A.d_real)
+        T::store4(row, dim, x[4 * q4] * scale, x[4 * q4 + 1] * scale, x[4 * q4 + 2] * scale,
+                  x[4 * q4 + 3] * scale);
+    }
+  }
+  // a key that met a non-finite value, again from its own rows (by one wave,
+  // after every wave's stores)
+  uint64_t any = __builtin_amdgcn_ballot_w64(bad && key_in);
+  any = (any | any >> 32) & 0xffffffffull;
+  if (lane < 32) met[wave][lane] = (uint32_t)(any >> lane) & 1u;
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  const bool fix = wave == 0 && (met[0][l32] | met[1][l32] | met[2][l32] | met[3][l32]);
+  fix_keys<E>(A, si, it.b, it.kvh, jw0, sink_end, fix, lane);
 }
 
 template <int D, Elem E>
@@ -539,19 +593,18 @@ hipError_t launch_bwd(const SinkArgs& a, hipStream_t stream) {
   sink_dq_kernel<D, E><<<(unsigned)n_dq, 256, 0, stream>>>(g);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int64_t units = (int64_t)a.n_sink_blocks * a.sink_chunks +
-                        (int64_t)(a.nkb - a.n_sink_blocks) * a.chunks;
+  int64_t units = 0, n_cut = 0;
+  for (int c = 0; c < 3; ++c) {
+    units += (int64_t)a.cls_n[c] * a.cls_cut[c];
+    n_cut += a.cls_cut[c] > 1 ? a.cls_n[c] : 0;
+  }
   const int64_t n_kv = (int64_t)a.B * a.Hkv * units;
   g.xcd_runs = sink_xcd_runs(a, n_kv);
   sink_dkdv_kernel<D, E><<<(unsigned)n_kv, 256, 0, stream>>>(g);
   e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  const int64_t n_cut = a.chunks > 1 ? a.nkb : a.n_sink_blocks;
-  if (n_cut > 0 && (a.chunks > 1 || a.sink_chunks > 1)) {
-    sink_join_kernel<D, E><<<(unsigned)(a.B * a.Hkv * n_cut), 256, 0, stream>>>(g);
-    e = hipGetLastError();
-  }
-  return e;
+  if (e != hipSuccess || n_cut == 0) return e;
+  sink_join_kernel<D, E><<<(unsigned)(4 * a.B * a.Hkv * n_cut), 256, 0, stream>>>(g);
+  return hipGetLastError();
 }
 
 template <Elem E>

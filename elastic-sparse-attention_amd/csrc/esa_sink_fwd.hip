@@ -18,31 +18,32 @@ namespace {
 
 template <int D, Elem E>
 struct SinkFwdCfg {
-  static constexpr int STAGE = E == Elem::f32 ? 32 : 64;  // keys
-  static constexpr int NB = STAGE / 32;
   static constexpr int WAVES_PER_SIMD = E == Elem::f32 ? 1 : 2;
 };
 
 template <int D, Elem E>
 __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_fwd_kernel(
     SinkArgs A) {
-  using C = SinkFwdCfg<D, E>;
   using T = SinkTile<D, E>;
-  using Stage = SinkStage<D, E, C::STAGE, 256>;
+  using Stage = SinkStage<D, E, 32, 256>;
   using LdsT = typename T::LdsT;
-  constexpr int ND = T::ND;
-  // separate objects, so that reads of one buffer are seen not to depend on
-  // the copies into the other
-  __shared__ __attribute__((aligned(1024))) LdsT k_st0[C::STAGE * D];
-  __shared__ __attribute__((aligned(1024))) LdsT v_st0[C::STAGE * D];
-  __shared__ __attribute__((aligned(1024))) LdsT k_st1[C::STAGE * D];
-  __shared__ __attribute__((aligned(1024))) LdsT v_st1[C::STAGE * D];
+  constexpr int ND = T::ND, N = 32 * D;
+  // four stages of 32 keys; separate objects, so that reads of one are seen
+  // not to depend on the copies into another
+  __shared__ __attribute__((aligned(1024))) LdsT k0_[N];
+  __shared__ __attribute__((aligned(1024))) LdsT v0_[N];
+  __shared__ __attribute__((aligned(1024))) LdsT k1_[N];
+  __shared__ __attribute__((aligned(1024))) LdsT v1_[N];
+  __shared__ __attribute__((aligned(1024))) LdsT k2_[N];
+  __shared__ __attribute__((aligned(1024))) LdsT v2_[N];
+  __shared__ __attribute__((aligned(1024))) LdsT k3_[N];
+  __shared__ __attribute__((aligned(1024))) LdsT v3_[N];
 
   const RowItem it = row_item(A);
   const int b = it.b, h = it.h, kvh = it.kvh, r0 = it.qb * 128;
   const SeqInfo si = seq_info(A, b);
   const int f = si.first, sink_end = min(f + A.sinks, A.kv_len), W = A.window;
-  const KeyStages keys = key_stages<C::STAGE>(A, si, r0, sink_end);
+  const KeyStages keys = key_stages<32>(A, si, r0, sink_end);
 
   const int tid = threadIdx.x;
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -52,6 +53,7 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
   const int p = si.base + r;
   const int pb = keys.pb, pw0 = si.base + r0 + wave * 32, pw1 = min(pw0 + 31, pb);
   const int n_all = keys.n_all;
+  const WaveStages ws = wave_stages<32>(keys, pw0, pw1, W, sink_end);
 
   T t;
   t.init(lane);
@@ -70,69 +72,170 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
   vs.init((const char*)A.v + ((int64_t)b * A.vsb + (int64_t)kvh * A.vsh) * T::ES, A.vss,
           A.kv_len, A.d_real, tid);
 
-  auto block = [&](const LdsT* kbuf, const LdsT* vbuf, int kb, int k0)
-                   __attribute__((always_inline)) {
-    if (pw0 > pb || none_seen(pw0, pw1, k0, W, sink_end)) return;
-    const bool full = all_seen(pw0, pw0 + 31, k0, W, sink_end);
-    f32x16 s = f32x16{};
-    if (!full) mask_init<0>(s, ~(seen_keys(p, k0, W, sink_end) >> (4 * hf)));
-    t.row_product(s, kbuf, kb, qf);
-    const float m_use = m_run == -INFINITY ? 0.f : m_run;
-    float smax = -INFINITY;
+  // Stages run as a pipeline: while a stage's scores go through the softmax
+  // and its product with V, the next stage's scores are formed, so the matrix
+  // pipe has work beside the exponentials.  s: the coming stage's scores (of
+  // the keys that the wave sees), top: each row's largest of them; used: the
+  // wave sees some of its keys.
+  f32x16 s = f32x16{};
+  float top = -INFINITY;
+  bool used = false;
+  auto row_top = [&](const f32x16& x) __attribute__((always_inline)) {
+    float y = fmaxf(x[0], x[1]);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[i] = __builtin_fmaf(s[i], scale, -m_use);
-      smax = fmaxf(smax, s[i]);
+    for (int i = 2; i < 16; ++i) y = fmaxf(y, x[i]);
+    return y;
+  };
+  auto hide = [&](f32x16& x, float& y, int i) __attribute__((always_inline)) {
+    if (!ws.full(i)) {
+      const int k0 = keys.key0(i);
+      uint32_t m[16];
+      key_masks<0>(m, seen_keys(p, k0, W, sink_end) >> (4 * hf));
+      mask_select(x, m);
+      y = row_top(x);
     }
-    smax = half_max(smax);
+  };
+  // stage i: its V in vbuf, the next stage's K in kbuf
+  auto step = [&](const LdsT* vbuf, const LdsT* kbuf, int i) __attribute__((always_inline)) {
+    const bool next = ws.sees(i + 1);
+    f32x16 sn = f32x16{};
+    if (!used) {
+      if (next) {
+        t.row_product(sn, kbuf, 0, qf);
+        top = row_top(sn);
+        hide(sn, top, i + 1);
+        s = sn;
+      }
+      used = next;
+      return;
+    }
+    top = half_max(top);
+    float m_use = m_run == -INFINITY ? 0.f : m_run;
     // the running maximum rises only past the slack (or at a row's first
     // visible key)
-    const float thr = m_run == -INFINITY ? -INFINITY : kRescaleSlack;
-    const bool grow = smax > thr;
+    const float over = __builtin_fmaf(top, scale, -m_use);
+    const bool grow = over > (m_run == -INFINITY ? -INFINITY : kRescaleSlack);
     if (wave_any(grow)) {
-      const float delta = grow ? smax : 0.f;
-      const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - (m_use + delta)) : 1.0f;
+      const float m_new = grow ? m_use + over : m_run;
+      const float alpha = grow ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.0f;
       l_run *= alpha;
       n_run *= alpha;
 #pragma unroll
       for (int d = 0; d < ND; ++d) oacc[d] *= alpha;
-      m_run = grow ? m_use + delta : m_run;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] -= delta;
+      m_run = m_new;
+      m_use = m_run == -INFINITY ? 0.f : m_run;
     }
+    // (past the wave's last key the product is of whatever the buffer holds,
+    // and dropped: no branch splits the scores from the softmax)
+    if constexpr (T::ES == 2) {
+      // in written order: products and exponentials side by side, V's reads
+      // ahead of the products that take them
+      typename T::V8 ka[T::NS];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[i] = __builtin_amdgcn_exp2f(s[i]);
-      l_run += s[i];
+      for (int k = 0; k < T::NS; ++k) ka[k] = t.row_operand(kbuf, 0, k);
+      u32x4 va[ND][2];
+      typename T::P pp;
+      auto exps = [&](int q) __attribute__((always_inline)) {  // two of the 16
+        s[2 * q] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * q], scale, -m_use));
+        s[2 * q + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * q + 1], scale, -m_use));
+        l_run += s[2 * q];
+        l_run += s[2 * q + 1];
+        pp.w[q] = T::M::pack2(s[2 * q], s[2 * q + 1]);
+      };
+      constexpr int H = T::NS / 2, EH = 4 / H > 0 ? 4 / H : 1;  // exponential pairs a product
+#pragma unroll
+      for (int k = 0; k < H; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        sn = T::M::mfma32(ka[k], qf.f[k], sn);
+        if (k < ND) va[k][0] = t.col_operand(vbuf, 0, k, 0);
+#pragma unroll
+        for (int e = 0; e < EH; ++e) exps(k * EH + e);
+      }
+#pragma unroll
+      for (int k = 0; k < H; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        sn = T::M::mfma32(ka[H + k], qf.f[H + k], sn);
+        if (k < ND) va[k][1] = t.col_operand(vbuf, 0, k, 1);
+#pragma unroll
+        for (int e = 0; e < EH; ++e) {
+          exps(4 + k * EH + e);
+          if (e == 0 && k < ND) t.col_step(oacc[k], va[k][0], pp, 0);
+        }
+      }
+      // O is normalised by the probabilities that its product used
+#pragma unroll
+      for (int k = 0; k < ND; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        t.col_step(oacc[k], va[k][1], pp, 1);
+        n_run = T::M::dot2(pp.w[2 * k], n_run);
+        n_run = T::M::dot2(pp.w[2 * k + 1], n_run);
+        if (ND == 2) {
+          n_run = T::M::dot2(pp.w[2 * k + 4], n_run);
+          n_run = T::M::dot2(pp.w[2 * k + 5], n_run);
+        }
+      }
+      top = row_top(sn);
+      __builtin_amdgcn_sched_barrier(0);
+    } else {
+      t.row_product(sn, kbuf, 0, qf);
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        s[k] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k], scale, -m_use));
+        l_run += s[k];
+      }
+      n_run = l_run;
+      t.col_product(oacc, vbuf, 0, t.pack(s));
+      top = row_top(sn);
     }
-    const typename T::P pp = t.pack(s);
-    // O is normalised by the probabilities that its product used
-    n_run = T::psum(pp, n_run);
-    t.col_product(oacc, vbuf, kb, pp);
+    if (next) hide(sn, top, i + 1);
+    s = sn;
+    used = next;
   };
-  auto stage = [&](const LdsT* kbuf, const LdsT* vbuf, int i) __attribute__((always_inline)) {
-    const int k0 = keys.key0(i);
-#pragma unroll
-    for (int kb = 0; kb < C::NB; ++kb) block(kbuf, vbuf, kb, k0 + 32 * kb);
+  // stage i's wait: its own loads and the next stage's have landed for every
+  // wave; the one after may be on its way
+  auto ready = [&](int i) __attribute__((always_inline)) {
+    if (i + 2 < n_all)
+      stage_wait<2 * Stage::LOADS>();
+    else
+      stage_wait<0>();
   };
+  auto issue = [&](int i, LdsT* kd, LdsT* vd) __attribute__((always_inline)) {
+    if (i < n_all) {
+      ks.issue(keys.key0(i), kd, wave);
+      vs.issue(keys.key0(i), vd, wave);
+    }
+  };
+  issue(0, k0_, v0_);
+  issue(1, k1_, v1_);
+  issue(2, k2_, v2_);
   if (n_all > 0) {
-    ks.issue(keys.key0(0), k_st0, wave);
-    vs.issue(keys.key0(0), v_st0, wave);
+    if (n_all > 2)
+      stage_wait<4 * Stage::LOADS>();
+    else
+      stage_wait<0>();
+    if (ws.sees(0)) {
+      t.row_product(s, k0_, 0, qf);
+      top = row_top(s);
+      hide(s, top, 0);
+      used = true;
+    }
   }
-  for (int i = 0; i < n_all; i += 2) {
-    stage_ready();
-    if (i + 1 < n_all) {
-      ks.issue(keys.key0(i + 1), k_st1, wave);
-      vs.issue(keys.key0(i + 1), v_st1, wave);
-    }
-    stage(k_st0, v_st0, i);
+  for (int i = 0; i < n_all; i += 4) {
+    ready(i);
+    issue(i + 3, k3_, v3_);
+    step(v0_, k1_, i);
     if (i + 1 >= n_all) break;
-    stage_ready();
-    if (i + 2 < n_all) {
-      ks.issue(keys.key0(i + 2), k_st0, wave);
-      vs.issue(keys.key0(i + 2), v_st0, wave);
-    }
-    stage(k_st1, v_st1, i + 1);
+    ready(i + 1);
+    issue(i + 4, k0_, v0_);
+    step(v1_, k2_, i + 1);
+    if (i + 2 >= n_all) break;
+    ready(i + 2);
+    issue(i + 5, k1_, v1_);
+    step(v2_, k3_, i + 2);
+    if (i + 3 >= n_all) break;
+    ready(i + 3);
+    issue(i + 6, k2_, v2_);
+    step(v3_, k0_, i + 3);
   }
 
   // ---- O rows and log-sum-exp
