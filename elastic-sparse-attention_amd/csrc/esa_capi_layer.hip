@@ -211,6 +211,7 @@ SinkArgs sink_fwd_args(const esa_fwd_args* a, const esa_window* w) {
   g.elem = a->dtype;
   g.sm_scale = a->sm_scale;
   g.scale_log2 = (float)((double)a->sm_scale * 1.4426950408889634);
+  g.ores = w->o_residual;
   sink_pattern(g, w);
   if (sink_decodes(g)) sink_splits(g);
   return g;
@@ -338,6 +339,7 @@ SinkArgs sink_bwd_args(const esa_bwd_args* a, const esa_window* w) {
   g.elem = a->dtype;
   g.sm_scale = a->sm_scale;
   g.scale_log2 = (float)((double)a->sm_scale * 1.4426950408889634);
+  g.ores = w->o_residual;
   sink_pattern(g, w);
   sink_bwd_plan(g);
   return g;
@@ -394,6 +396,7 @@ esa_status esa_sink_window_fwd(const esa_fwd_args* a, const esa_window* w, void*
       (s = sink_rows_ok(a->v, a->v_stride_b, a->v_stride_h, a->v_stride_s, epc)) != ESA_OK ||
       (s = sink_rows_ok(a->o, a->o_stride_b, a->o_stride_h, a->o_stride_s, epc)) != ESA_OK)
     return s;
+  if (!aligned(w->o_residual, 16)) return ESA_ERR_ALIGN;
   SinkArgs g = sink_fwd_args(a, w);
   const size_t need = sink_fwd_workspace(g);
   if (need > 0) {
@@ -438,6 +441,7 @@ esa_status esa_sink_window_bwd(const esa_bwd_args* a, const esa_window* w, void*
       (s = sink_rows_ok(a->dk, a->dk_stride_b, a->dk_stride_h, a->dk_stride_s, epc)) != ESA_OK ||
       (s = sink_rows_ok(a->dv, a->dv_stride_b, a->dv_stride_h, a->dv_stride_s, epc)) != ESA_OK)
     return s;
+  if (!aligned(w->o_residual, 16)) return ESA_ERR_ALIGN;
   SinkArgs g = sink_bwd_args(a, w);
   const SinkBwdSizes z = sink_bwd_sizes(g);
   if (!workspace) return ESA_ERR_NULL;

@@ -15,6 +15,7 @@ struct SinkArgs {
   const void *q, *k, *v;
   void* o;
   float* lse;
+  void* ores;  // what rounding o lost, in o's type and layout, or NULL
   const void* dout;
   void *dq, *dk, *dv;
   int64_t qsb, qsh, qss, ksb, ksh, kss, vsb, vsh, vss, osb, osh, oss, lsb, lsh;
@@ -284,6 +285,7 @@ struct SinkTile {
     v[3] = (typename M::s)e;
     *(typename M::v4*)((uint16_t*)row + dim) = v;
   }
+  static __device__ __forceinline__ float rounded(float x) { return (float)(typename M::s)x; }
   static __device__ __forceinline__ float psum(const P& p, float c) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) c = M::dot2(p.w[q], c);
@@ -356,6 +358,7 @@ struct SinkTile<D, Elem::f32, TIGHT> {
                                                 float e) {
     *(f32x4*)((float*)row + dim) = f32x4{a, b, c, e};
   }
+  static __device__ __forceinline__ float rounded(float x) { return x; }
   static __device__ __forceinline__ float psum(const P& p, float c) {
 #pragma unroll
     for (int q = 0; q < 16; ++q) c += p[q];
@@ -476,6 +479,18 @@ __device__ __forceinline__ float row_dot(const void* a, const void* b, int d_rea
   return s;
 }
 
+// Four dims of an output row, and (where the caller keeps it for a backward)
+// what rounding them lost.
+template <int D, Elem E>
+__device__ __forceinline__ void store_out4(const SinkArgs& A, int64_t row, int dim, float a,
+                                           float b, float c, float d) {
+  using T = SinkTile<D, E>;
+  T::store4((char*)A.o + row * T::ES, dim, a, b, c, d);
+  if (A.ores)
+    T::store4((char*)A.ores + row * T::ES, dim, a - T::rounded(a), b - T::rounded(b),
+              c - T::rounded(c), d - T::rounded(d));
+}
+
 // Row `row` of one head from its own keys, by one wave: lanes take 64 keys at a
 // time for the scores and the head's dims for the weighted sum.
 template <Elem E>
@@ -513,10 +528,15 @@ __device__ void fix_row(const SinkArgs& A, int b, int h, int kvh, int row, int p
     }
   }
   const bool empty = rk.n <= 0;
-  EL* o = (EL*)A.o + (int64_t)b * A.osb + (int64_t)h * A.osh + (int64_t)row * A.oss;
+  const int64_t at = (int64_t)b * A.osb + (int64_t)h * A.osh + (int64_t)row * A.oss;
 #pragma unroll
   for (int c = 0; c < 2; ++c)
-    if (lane + 64 * c < A.d_real) T::store(o + lane + 64 * c, empty ? 0.f : acc[c] / l);
+    if (lane + 64 * c < A.d_real) {
+      const float y = empty ? 0.f : acc[c] / l;
+      EL* o = (EL*)A.o + at + lane + 64 * c;
+      T::store(o, y);
+      if (A.ores) T::store((EL*)A.ores + at + lane + 64 * c, y - T::load(o));
+    }
   if (A.lse && lane == 0)
     A.lse[(int64_t)b * A.lsb + (int64_t)h * A.lsh + row] =
         empty ? -INFINITY : (m + __log2f(l)) * 0.69314718055994530942f;

@@ -5,7 +5,10 @@
 //   dS = P * (dP - delta),  delta = rowsum(dO * O),
 //   dQ = scale dS K,  dK = scale dS^T Q
 //
-//   sink_prep_kernel  delta and lse in log2 units, one 16-lane group a row
+//   sink_prep_kernel  delta and lse in log2 units, one 16-lane group a row (from
+//                     O as it was before its rounding, where the forward kept
+//                     the difference: a rounded O alone leaves dQ and dK about
+//                     8% further off)
 //   sink_dq_kernel    128 rows a workgroup, over the keys they see, as the
 //                     forward: S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T
 //   sink_dkdv_kernel  128 keys a workgroup, over the rows that see them: the
@@ -52,12 +55,16 @@ __global__ __launch_bounds__(256) void sink_prep_kernel(SinkArgs A) {
     const int r = (int)(id - bh * A.q_len);
     const int b = (int)(bh / A.H), h = (int)(bh - (int64_t)b * A.H);
     const auto* o = at<E>(A.o, (int64_t)b * A.osb + (int64_t)h * A.osh + (int64_t)r * A.oss);
+    const auto* res = at<E>(A.ores, (int64_t)b * A.osb + (int64_t)h * A.osh + (int64_t)r * A.oss);
     const auto* d = at<E>(A.dout, (int64_t)b * A.dosb + (int64_t)h * A.dosh + (int64_t)r * A.doss);
     float acc = 0.f;
     for (int c = g * T::kPerChunk; c < A.d_real; c += 16 * T::kPerChunk) {
       const u32x4 x = *(const u32x4*)(o + c), y = *(const u32x4*)(d + c);
+      u32x4 z = {0u, 0u, 0u, 0u};
+      if (A.ores) z = *(const u32x4*)(res + c);
 #pragma unroll
-      for (int e = 0; e < T::kPerChunk; ++e) acc = __builtin_fmaf(T::chunk(x, e), T::chunk(y, e), acc);
+      for (int e = 0; e < T::kPerChunk; ++e)
+        acc = __builtin_fmaf(T::chunk(x, e) + T::chunk(z, e), T::chunk(y, e), acc);
     }
 #pragma unroll
     for (int off = 8; off >= 1; off >>= 1) acc += __shfl_xor(acc, off, 16);

@@ -263,7 +263,7 @@ __global__ __launch_bounds__(256, 2) void sink_decode_kernel(SinkArgs A) {
   const bool whole = A.splits == 1;
   const float inv = whole ? (pj < f ? 0.f : 1.f / nt) : 1.f;
   const bool valid = jin && (!whole || row_valid(A, si, b, jrow.s));
-  EL* orow = (EL*)A.o + (int64_t)b * A.osb + (int64_t)jrow.h * A.osh + (int64_t)jrow.s * A.oss;
+  const int64_t orow = (int64_t)b * A.osb + (int64_t)jrow.h * A.osh + (int64_t)jrow.s * A.oss;
   const int64_t unit = (int64_t)blockIdx.x * 16 + jr;
   bool finite = true;
 #pragma unroll
@@ -278,7 +278,7 @@ __global__ __launch_bounds__(256, 2) void sink_decode_kernel(SinkArgs A) {
     if (!jin || dim >= A.d_real) continue;
     if (whole) {
       if (!valid) y = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
-      SinkTile<D, E>::store4(orow, dim, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+      store_out4<D, E>(A, orow, dim, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
     } else {
       *(f32x4*)(A.partial + unit * D + dim) = y;
     }
@@ -358,13 +358,13 @@ __global__ __launch_bounds__(256) void sink_decode_join_kernel(SinkArgs A) {
   }
   const bool valid = row_valid(A, si, b, row.s);
   const float inv = !valid ? __builtin_nanf("") : p < f ? 0.f : 1.f / nt;
-  EL* orow = (EL*)A.o + (int64_t)b * A.osb + (int64_t)row.h * A.osh + (int64_t)row.s * A.oss;
+  const int64_t orow = (int64_t)b * A.osb + (int64_t)row.h * A.osh + (int64_t)row.s * A.oss;
   bool finite = true;
   if (lane < LPR && 4 * lane < A.d_real) {
     f32x4 z = {0.f, 0.f, 0.f, 0.f};
     for (int q = 0; q < GR; ++q) z += *(const f32x4*)(ob[q] + 4 * lane);
     finite = __builtin_isfinite((z[0] + z[1]) + (z[2] + z[3]));
-    SinkTile<D, E>::store4(orow, 4 * lane, z[0] * inv, z[1] * inv, z[2] * inv, z[3] * inv);
+    store_out4<D, E>(A, orow, 4 * lane, z[0] * inv, z[1] * inv, z[2] * inv, z[3] * inv);
   }
   if (A.lse && lane == 0)
     A.lse[(int64_t)b * A.lsb + (int64_t)row.h * A.lsh + row.s] =

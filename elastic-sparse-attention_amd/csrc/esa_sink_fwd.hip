@@ -252,16 +252,15 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
       lse = -INFINITY;
     }
     if (!valid) inv = lse = __builtin_nanf("");
-    char* orow = (char*)A.o + ((int64_t)b * A.osb + (int64_t)h * A.osh + (int64_t)r * A.oss) *
-                                  T::ES;
+    const int64_t orow = (int64_t)b * A.osb + (int64_t)h * A.osh + (int64_t)r * A.oss;
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
         const int dim = 32 * d + 8 * q4 + 4 * hf;
         if (dim < A.d_real)
-          T::store4(orow, dim, oacc[d][4 * q4] * inv, oacc[d][4 * q4 + 1] * inv,
-                    oacc[d][4 * q4 + 2] * inv, oacc[d][4 * q4 + 3] * inv);
+          store_out4<D, E>(A, orow, dim, oacc[d][4 * q4] * inv, oacc[d][4 * q4 + 1] * inv,
+                           oacc[d][4 * q4 + 2] * inv, oacc[d][4 * q4 + 3] * inv);
       }
     if (A.lse && hf == 0) A.lse[(int64_t)b * A.lsb + (int64_t)h * A.lsh + r] = lse;
   }

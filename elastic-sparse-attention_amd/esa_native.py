@@ -116,6 +116,7 @@ class EsaWindow(ctypes.Structure):
         ("positions", ctypes.c_void_p),
         ("position_stride_b", ctypes.c_int64),
         ("first_key", ctypes.c_void_p),
+        ("o_residual", ctypes.c_void_p),
     ]
 
 

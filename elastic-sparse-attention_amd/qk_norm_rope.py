@@ -24,7 +24,6 @@ hand-written gfx950 kernels; CPU tensors raise.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from typing import Optional, Tuple
 
@@ -37,12 +36,20 @@ from esa_native import EsaRotaryArgs, check, load
 __all__ = ["QKNormRope", "qk_norm_rope_fwd", "qk_norm_rope_bwd", "qk_norm_rope_append"]
 
 
-def _on(device: torch.device):
-    """The device of a call's tensors made current, where it is another one:
-    a launch goes to the current device."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+_GET_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _launch(device: torch.device, what: str, fn, *args) -> None:
+    """``fn(*args, stream)`` on the device's current stream, the device made
+    current where it is another one (a launch goes to the current device)."""
+    index = device.index
+    if index is None or index == _GET_DEVICE():
+        status = fn(*args, _stream(device))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _stream(device))
+    if status:
+        check(status, what)
 
 
 def _like(t: torch.Tensor) -> torch.Tensor:
@@ -96,7 +103,7 @@ def _weights(q_weight, k_weight, D: int, device: torch.device):
                 raise ValueError(f"{name} must be [{D}], got {list(w.shape)}")
             if w.device != device:
                 raise ValueError(f"{name} is on {w.device}, the rows are on {device}")
-            w = w.detach().contiguous()
+            w = w.detach() if w.is_contiguous() else w.detach().contiguous()
         out.append(w)
     qw, kw = out
     if qw is not None and kw is not None and qw.dtype != kw.dtype:
@@ -104,32 +111,36 @@ def _weights(q_weight, k_weight, D: int, device: torch.device):
     return qw, kw
 
 
-def _rotary_args(q, k, q_weight, k_weight, inv_freq, pos, eps, interleaved) -> EsaRotaryArgs:
-    B, H, n, D = q.shape
-    w = q_weight if q_weight is not None else k_weight
-    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.device != q.device:
-        raise ValueError("inv_freq must be a 1-D float64 tensor on the rows' device")
-    a = EsaRotaryArgs()
-    a.dtype = _dtype_code(q.dtype)
-    a.weight_dtype = _dtype_code(w.dtype) if w is not None else a.dtype
-    a.batch, a.num_heads, a.num_kv_heads, a.seq_len, a.head_dim = B, H, k.shape[1], n, D
-    a.rotary_dim = 2 * inv_freq.shape[0]
-    a.interleaved = 1 if interleaved else 0
-    a.eps = float(eps)
-    a.q_weight = q_weight.data_ptr() if q_weight is not None else None
-    a.k_weight = k_weight.data_ptr() if k_weight is not None else None
-    a.inv_freq = inv_freq.data_ptr()
-    a.positions = pos.data_ptr()
-    a.position_stride_b = pos.stride(0) if pos.dim() == 2 and pos.shape[0] > 1 else 0
-    return a
+_NO_TENSOR = (None, 0, 0, 0)
 
 
-def _set(a: EsaRotaryArgs, name: str, t: torch.Tensor) -> None:
+def _rows_of(t: Optional[torch.Tensor]):
+    """Address and (b, h, s) strides, in the order of esa_rotary_args."""
+    if t is None:
+        return _NO_TENSOR
     st = t.stride()
-    setattr(a, name, t.data_ptr())
-    setattr(a, name + "_stride_b", st[0])
-    setattr(a, name + "_stride_h", st[1])
-    setattr(a, name + "_stride_s", st[2])
+    return t.data_ptr(), st[0], st[1], st[2]
+
+
+def _rotary_args(q, k, v, q_out, k_out, v_out, q_grad, k_grad, q_weight, k_weight, inv_freq, pos,
+                 eps, interleaved, kv_len=0, dq_weight=None, dk_weight=None) -> EsaRotaryArgs:
+    B, H, n, D = q.shape
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or inv_freq.device != q.device \
+            or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous 1-D float64 tensor on the rows' device")
+    code = _dtype_code(q.dtype)
+    w = q_weight if q_weight is not None else k_weight
+    # in the order of esa_rotary_args' fields
+    return EsaRotaryArgs(
+        code, code if w is None else _dtype_code(w.dtype), B, H, k.shape[1], n, D,
+        2 * inv_freq.shape[0], 1 if interleaved else 0, kv_len, eps,
+        None if q_weight is None else q_weight.data_ptr(),
+        None if k_weight is None else k_weight.data_ptr(), inv_freq.data_ptr(), pos.data_ptr(),
+        pos.stride(0) if pos.dim() == 2 and pos.shape[0] > 1 else 0,
+        *_rows_of(q), *_rows_of(k), *_rows_of(v), *_rows_of(q_out), *_rows_of(k_out),
+        *_rows_of(v_out), *_rows_of(q_grad), *_rows_of(k_grad),
+        None if dq_weight is None else dq_weight.data_ptr(),
+        None if dk_weight is None else dk_weight.data_ptr())
 
 
 def _align(t: torch.Tensor) -> int:
@@ -152,13 +163,10 @@ def qk_norm_rope_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.
     pos = _positions_2d(positions, B, n, q.device)
     qw, kw = _weights(q_weight, k_weight, D, q.device)
     qo, ko = _like(q), _like(k)
-    q, k = _prep(q, _align(q)), _prep(k, _align(k))
-    a = _rotary_args(q, k, qw, kw, inv_freq.contiguous(), pos, eps, interleaved)
-    for name, t in (("q", q), ("k", k), ("q_out", qo), ("k_out", ko)):
-        _set(a, name, t)
-    with _on(q.device):
-        check(load().esa_qk_norm_rope_fwd(ctypes.byref(a), _stream(q.device)),
-              "esa_qk_norm_rope_fwd")
+    align = _align(q)
+    a = _rotary_args(_prep(q, align), _prep(k, align), None, qo, ko, None, None, None, qw, kw,
+                     inv_freq, pos, eps, interleaved)
+    _launch(q.device, "esa_qk_norm_rope_fwd", load().esa_qk_norm_rope_fwd, ctypes.byref(a))
     return qo, ko
 
 
@@ -179,26 +187,22 @@ def qk_norm_rope_bwd(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.
     pos = _positions_2d(positions, B, n, q.device)
     qw, kw = _weights(q_weight, k_weight, D, q.device)
     dq, dk = _like(q), _like(k)
-    q, k = _prep(q, _align(q)), _prep(k, _align(k))
-    gq, gk = (_prep(g.to(device=q.device, dtype=q.dtype), _align(q)) for g in (dq_out, dk_out))
-    a = _rotary_args(q, k, qw, kw, inv_freq.contiguous(), pos, eps, interleaved)
-    for name, t in (("q", q), ("k", k), ("q_out", dq), ("k_out", dk), ("q_grad", gq),
-                    ("k_grad", gk)):
-        _set(a, name, t)
     dqw = torch.empty_like(qw) if weight_grads and qw is not None else None
     dkw = torch.empty_like(kw) if weight_grads and kw is not None else None
     if B == 0 or n == 0:  # no rows: nothing is launched
         return dq, dk, *(None if w is None else w.zero_() for w in (dqw, dkw))
-    a.q_weight_grad = dqw.data_ptr() if dqw is not None else None
-    a.k_weight_grad = dkw.data_ptr() if dkw is not None else None
+    align = _align(q)
+    q, k = _prep(q, align), _prep(k, align)
+    gq, gk = (_prep(g.to(device=q.device, dtype=q.dtype), align) for g in (dq_out, dk_out))
+    a = _rotary_args(q, k, None, dq, dk, None, gq, gk, qw, kw, inv_freq, pos, eps, interleaved, 0,
+                     dqw, dkw)
     lib = load()
     ws = ctypes.c_size_t()
     check(lib.esa_qk_norm_rope_bwd_workspace_size(ctypes.byref(a), ctypes.byref(ws)),
           "esa_qk_norm_rope_bwd_workspace_size")
     work = torch.empty(max(ws.value, 16), dtype=torch.uint8, device=q.device)
-    with _on(q.device):
-        check(lib.esa_qk_norm_rope_bwd(ctypes.byref(a), work.data_ptr(), work.numel(),
-                                       _stream(q.device)), "esa_qk_norm_rope_bwd")
+    _launch(q.device, "esa_qk_norm_rope_bwd", lib.esa_qk_norm_rope_bwd, ctypes.byref(a),
+            work.data_ptr(), work.numel())
     return dq, dk, dqw, dkw
 
 
@@ -220,21 +224,21 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     _require_gpu(v, k_cache, v_cache)
     B, _, n, D = q.shape
     Hkv = k.shape[1]
+    align = _align(q)
     if v.shape != k.shape:
         raise ValueError(f"key {tuple(k.shape)} and value {tuple(v.shape)} shapes differ")
     for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if c.dim() != 4 or c.shape[0] != B or c.shape[1] != Hkv or c.shape[3] != D:
-            raise ValueError(f"{name} must be [{B}, {Hkv}, Lmax, {D}], got {list(c.shape)}")
+        cs, st = c.shape, c.stride()
+        if len(cs) != 4 or cs[0] != B or cs[1] != Hkv or cs[3] != D:
+            raise ValueError(f"{name} must be [{B}, {Hkv}, Lmax, {D}], got {list(cs)}")
         if c.dtype != q.dtype or c.device != q.device:
             raise ValueError(f"{name} must have the rows' dtype and device")
-        if c.shape[2] > 1 and B * Hkv > 0 and 0 in c.stride()[:3]:
-            if any(s == 0 and m > 1 for s, m in zip(c.stride(), c.shape)):
-                raise ValueError(f"{name} is an expanded view: its rows share memory")
-        al = _align(c)
-        if c.stride(3) != 1 or c.data_ptr() % (al * c.element_size()) or \
-                any(s % al for s in c.stride()[:3]):
+        if 0 in st and any(x == 0 and m > 1 for x, m in zip(st, cs)):
+            raise ValueError(f"{name} is an expanded view: its rows share memory")
+        if st[3] != 1 or (st[0] | st[1] | st[2]) & (align - 1) or \
+                c.data_ptr() % (align * c.element_size()):
             raise ValueError(f"{name} is written in place: its rows must be contiguous and "
-                             f"aligned to {al * c.element_size()} bytes")
+                             f"aligned to {align * c.element_size()} bytes")
     if k_cache.shape[2] != v_cache.shape[2]:
         raise ValueError("k_cache and v_cache differ in length")
     if v.dtype != q.dtype or v.device != q.device:
@@ -247,15 +251,9 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         return qo
     if Lmax == 0:
         return qo.fill_(float("nan"))
-    q, k, v = (_prep(t, _align(t)) for t in (q, k, v))
-    a = _rotary_args(q, k, qw, kw, inv_freq.contiguous(), pos, eps, interleaved)
-    a.kv_len = Lmax
-    for name, t in (("q", q), ("k", k), ("v", v), ("q_out", qo), ("k_out", k_cache),
-                    ("v_out", v_cache)):
-        _set(a, name, t)
-    with _on(q.device):
-        check(load().esa_qk_norm_rope_append(ctypes.byref(a), _stream(q.device)),
-              "esa_qk_norm_rope_append")
+    a = _rotary_args(_prep(q, align), _prep(k, align), _prep(v, align), qo, k_cache, v_cache, None,
+                     None, qw, kw, inv_freq, pos, eps, interleaved, Lmax)
+    _launch(q.device, "esa_qk_norm_rope_append", load().esa_qk_norm_rope_append, ctypes.byref(a))
     return qo
 
 

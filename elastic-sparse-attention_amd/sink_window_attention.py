@@ -27,23 +27,24 @@ from typing import Optional, Tuple
 import torch
 import torch.nn as nn
 
-from elastic_sparse_attention import (_bwd_args, _check_qkv, _fwd_args, _prep, _require_gpu,
-                                      _stream)
-from esa_native import EsaWindow, check, load
-from qk_norm_rope import _like, _on, check_cache_position
+from elastic_sparse_attention import (_check_qkv, _dtype_code, _fwd_args, _prep, _require_gpu)
+from esa_native import EsaBwdArgs, EsaWindow, check, load
+from qk_norm_rope import _launch, _like, check_cache_position
 
 __all__ = ["SinkWindowAttention", "sink_window_attention_fwd", "sink_window_attention_bwd"]
 
 
 def _window(window: int, sinks: int, positions: Optional[torch.Tensor],
-            first_key: Optional[torch.Tensor]) -> EsaWindow:
+            first_key: Optional[torch.Tensor],
+            residual: Optional[torch.Tensor] = None) -> EsaWindow:
     pos_ptr = pos_sb = 0
     if positions is not None:
         pos_ptr = positions.data_ptr()
         if positions.dim() == 2 and positions.shape[0] > 1:
             pos_sb = positions.stride(0)
     return EsaWindow(min(window, 0x7fffffff), min(sinks, 0x7fffffff), pos_ptr or None, pos_sb,
-                     None if first_key is None else first_key.data_ptr())
+                     None if first_key is None else first_key.data_ptr(),
+                     None if residual is None else residual.data_ptr())
 
 
 def _check_window(window: int, sinks: int) -> None:
@@ -68,7 +69,8 @@ def _first_keys(first_key, batch: int, device: torch.device) -> Optional[torch.T
 
 
 def _checked(q, k, v, positions, first_key):
-    _check_qkv(q, k, v)
+    """positions and first_key as the kernels take them (q, k, v having passed
+    _check_qkv)."""
     if not (q.device == k.device == v.device):
         raise ValueError(f"q, k and v must share one device, got {q.device}, {k.device} and "
                          f"{v.device}")
@@ -84,8 +86,7 @@ def _checked(q, k, v, positions, first_key):
 
 def sink_window_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int,
                               num_sinks: int, scaling: float, positions=None, first_key=None,
-                              return_lse: bool = True
-                              ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+                              return_lse: bool = True, return_residual: bool = False):
     """``o`` as ``[B, Lq, H, D]`` and, if asked, ``lse`` float32 ``[B, H, Lq]``
     (natural log).
 
@@ -94,48 +95,67 @@ def sink_window_attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     is checked, a device tensor used as given: a row that breaks this, or lies
     outside the cache, gives NaN).  ``first_key``: None or int ``[B]``, the
     first key of each sequence (left padding); rows before it give 0 and
-    lse -inf."""
+    lse -inf.  ``return_residual`` adds a third value for the backward: what
+    rounding o to 16 bits lost (None for float32)."""
+    _check_qkv(q, k, v)
     positions, first_key = _checked(q, k, v, positions, first_key)
     _check_window(window, num_sinks)
-    return _fwd(q, k, v, window, num_sinks, scaling, positions, first_key, return_lse)
+    got = _fwd(q, k, v, window, num_sinks, scaling, positions, first_key, return_lse,
+               return_residual)
+    return got if return_residual else got[:2]
 
 
-def _fwd(q, k, v, window, sinks, scaling, positions, first_key, return_lse):
-    """The forward after its checks (the module makes them itself)."""
+# workspace bytes of the forward by its shape (a question to the library that
+# a decode step need not ask again)
+_WORKSPACE = {}
+
+
+def _fwd(q, k, v, window, sinks, scaling, positions, first_key, return_lse, residual=False):
+    """The forward after its checks (the module makes them itself): o, lse and,
+    for a backward, what rounding o lost (None for float32)."""
     B, H, Lq, D = q.shape
     device = q.device
     align = 16 // q.element_size()
     o = torch.empty((B, Lq, H, D), dtype=q.dtype, device=device)
     lse = torch.empty((B, H, Lq), dtype=torch.float32, device=device) if return_lse else None
+    res = torch.empty_like(o) if residual and o.dtype != torch.float32 else None
     if B == 0 or Lq == 0:
-        return o, lse
+        return o, lse, res
     if k.shape[2] == 0:  # every row lies outside an empty cache
         o.fill_(float("nan"))
-        return o, None if lse is None else lse.fill_(float("nan"))
+        return o, None if lse is None else lse.fill_(float("nan")), res
     q, k, v = _prep(q, align), _prep(k, align), _prep(v, align)
     a = _fwd_args(q, k, v, o, (Lq * H * D, D, H * D), lse, scaling)
-    w = _window(window, sinks, positions, first_key)
+    w = _window(window, sinks, positions, first_key, res)
     lib = load()
-    ws = ctypes.c_size_t()
-    check(lib.esa_sink_window_fwd_workspace_size(ctypes.byref(a), ctypes.byref(w),
-                                                 ctypes.byref(ws)),
-          "esa_sink_window_fwd_workspace_size")
-    n = ws.value
+    key = (B, H, k.shape[1], Lq, k.shape[2], D, q.dtype, window, sinks, positions is None)
+    n = _WORKSPACE.get(key)
+    if n is None:
+        ws = ctypes.c_size_t()
+        check(lib.esa_sink_window_fwd_workspace_size(ctypes.byref(a), ctypes.byref(w),
+                                                     ctypes.byref(ws)),
+              "esa_sink_window_fwd_workspace_size")
+        n = ws.value
+        if len(_WORKSPACE) >= 4096:
+            _WORKSPACE.clear()
+        _WORKSPACE[key] = n
     work = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-    with _on(device):
-        check(lib.esa_sink_window_fwd(ctypes.byref(a), ctypes.byref(w),
-                                      work.data_ptr() if n else None, n, _stream(device)),
-              "esa_sink_window_fwd")
-    return o, lse
+    _launch(device, "esa_sink_window_fwd", lib.esa_sink_window_fwd, ctypes.byref(a),
+            ctypes.byref(w), work.data_ptr() if n else None, n)
+    return o, lse, res
 
 
 def sink_window_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor,
                               lse: torch.Tensor, dout: torch.Tensor, window: int, num_sinks: int,
-                              scaling: float, positions=None, first_key=None
+                              scaling: float, positions=None, first_key=None,
+                              o_residual: Optional[torch.Tensor] = None
                               ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``dq``, ``dk``, ``dv`` in the inputs' shapes and dtype from the
     forward's ``o`` and ``dout`` ``[B, Lq, H, D]`` and ``lse``; sums in a fixed
-    order, no atomics."""
+    order, no atomics.  ``o_residual``: the forward's third value, with which
+    dq and dk come out closer (rowsum(dout * o) from the o before its
+    rounding); the module's backward has it."""
+    _check_qkv(q, k, v)
     positions, first_key = _checked(q, k, v, positions, first_key)
     _check_window(window, num_sinks)
     B, H, Lq, D = q.shape
@@ -145,25 +165,46 @@ def sink_window_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     _require_gpu(o, lse, dout)
     if o.dtype != q.dtype or lse.dtype != torch.float32:
         raise ValueError("o must have q's dtype and lse float32, as the forward returns them")
+    if o_residual is not None:
+        if o_residual.shape != o.shape or o_residual.dtype != o.dtype or \
+                o_residual.device != o.device:
+            raise ValueError("o_residual must have o's shape, dtype and device")
+        o, o_residual = _prep(o.contiguous(), 8), _prep(o_residual.contiguous(), 8)
+    return _bwd(q, k, v, o, lse, dout, window, num_sinks, scaling, positions, first_key,
+                o_residual)
+
+
+def _rows_of(t: torch.Tensor, order=(0, 1, 2)):
+    st = t.stride()
+    return t.data_ptr(), st[order[0]], st[order[1]], st[order[2]]
+
+
+def _bwd(q, k, v, o, lse, dout, window, sinks, scaling, positions, first_key, residual):
+    """The backward after its checks (o contiguous where residual is given)."""
+    B, H, Lq, D = q.shape
     dq, dk, dv = _like(q), _like(k), _like(v)
     if B == 0 or Lq == 0 or k.shape[2] == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()  # no query row reaches a key
     align = 16 // q.element_size()
-    q, k, v, o = (_prep(t, align) for t in (q, k, v, o))
-    dout = _prep(dout.to(q.dtype), align)
+    q, k, v, o = _prep(q, align), _prep(k, align), _prep(v, align), _prep(o, align)
+    dout = _prep(dout if dout.dtype == q.dtype else dout.to(q.dtype), align)
     lse = lse.contiguous()
-    a = _bwd_args(q, k, v, o, (o.stride(0), o.stride(2), o.stride(1)), lse, dout,
-                  (dout.stride(0), dout.stride(2), dout.stride(1)), dq, dk, dv, scaling)
-    w = _window(window, num_sinks, positions, first_key)
+    bshd = (0, 2, 1)
+    # in the order of esa_bwd_args' fields
+    a = EsaBwdArgs(_dtype_code(q.dtype), B, H, k.shape[1], Lq, k.shape[2], D, *_rows_of(q),
+                   *_rows_of(k), *_rows_of(v), *_rows_of(o, bshd), *_rows_of(dout, bshd),
+                   *_rows_of(dq), *_rows_of(dk), *_rows_of(dv), lse.data_ptr(), lse.stride(0),
+                   lse.stride(1), float(scaling))
+    w = _window(window, sinks, positions, first_key, residual)
     lib = load()
     ws = ctypes.c_size_t()
     check(lib.esa_sink_window_bwd_workspace_size(ctypes.byref(a), ctypes.byref(w),
                                                  ctypes.byref(ws)),
           "esa_sink_window_bwd_workspace_size")
-    work = torch.empty(ws.value, dtype=torch.uint8, device=q.device)
-    with _on(q.device):
-        check(lib.esa_sink_window_bwd(ctypes.byref(a), ctypes.byref(w), work.data_ptr(), ws.value,
-                                      _stream(q.device)), "esa_sink_window_bwd")
+    n = ws.value
+    work = torch.empty(n, dtype=torch.uint8, device=q.device)
+    _launch(q.device, "esa_sink_window_bwd", lib.esa_sink_window_bwd, ctypes.byref(a),
+            ctypes.byref(w), work.data_ptr(), n)
     return dq, dk, dv
 
 
@@ -173,16 +214,16 @@ class _SinkWindowFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, window, num_sinks, scaling, positions, first_key):
-        o, lse = _fwd(q, k, v, window, num_sinks, scaling, positions, first_key, True)
-        ctx.save_for_backward(q, k, v, o, lse, positions, first_key)
+        o, lse, res = _fwd(q, k, v, window, num_sinks, scaling, positions, first_key, True, True)
+        ctx.save_for_backward(q, k, v, o, lse, res, positions, first_key)
         ctx.window, ctx.num_sinks, ctx.scaling = window, num_sinks, scaling
         return o
 
     @staticmethod
     def backward(ctx, do):
-        q, k, v, o, lse, positions, first_key = ctx.saved_tensors
-        dq, dk, dv = sink_window_attention_bwd(q, k, v, o, lse, do, ctx.window, ctx.num_sinks,
-                                               ctx.scaling, positions, first_key)
+        q, k, v, o, lse, res, positions, first_key = ctx.saved_tensors
+        dq, dk, dv = _bwd(q, k, v, o, lse, do, ctx.window, ctx.num_sinks, ctx.scaling, positions,
+                          first_key, res)
         return dq, dk, dv, None, None, None, None, None
 
 
@@ -262,7 +303,7 @@ class SinkWindowAttention(nn.Module):
             o = _SinkWindowFunction.apply(q, k, v, self.window, self.num_sinks, self.scaling,
                                           positions, first_key)
         else:
-            o, _ = _fwd(q, k, v, self.window, self.num_sinks, self.scaling, positions, first_key,
-                        False)
+            o = _fwd(q, k, v, self.window, self.num_sinks, self.scaling, positions, first_key,
+                     False)[0]
         B, Lq, H, D = o.shape
         return o.view(B, Lq, H * D), None

@@ -596,6 +596,9 @@ typedef struct esa_window {
   const int64_t* positions;  /* device, [q_len] a sequence, or NULL */
   int64_t position_stride_b; /* 0: shared by the batch */
   const int64_t* first_key;  /* device, [batch], or NULL */
+  /* NULL, or memory of o's type and strides: the forward leaves there what
+   * rounding o lost, the backward takes it into delta = rowsum(dout * o) */
+  void* o_residual;
 } esa_window;
 
 /* Host only.  Workspace of esa_sink_window_fwd: 0 but for a few rows against

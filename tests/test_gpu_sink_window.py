@@ -194,6 +194,34 @@ def test_rows_of_a_cache(B, H, Hkv, Lq, Lk, D, W, S, dtype, start, first):
         close(got, r, t, what)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("Lq,Lk", [(0, 260), (1, 700), (1, 20), (4, 300)])
+def test_residual_of_o(dtype, Lq, Lk):
+    """o plus its residual is the output in nearly twice the bits: off by the
+    float32 sums' and the probabilities' error alone, which is common to both."""
+    B, H, Hkv, D, W, S = 2, 4, 2, 64, 100, 3
+    n = Lq or Lk
+    q, k, v, gen = make(B, H, Hkv, n, Lk, D, dtype, False, 7)
+    pos = None if not Lq else torch.tensor([Lk - n, 9])[:, None] + torch.arange(n)
+    qd, kd, vd = q.to(DEV), k.to(DEV), v.to(DEV)
+    o, lse, res = sink_window_attention_fwd(qd, kd, vd, W, S, 0.125, pos, return_residual=True)
+    o2, lse2 = sink_window_attention_fwd(qd, kd, vd, W, S, 0.125, pos)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    assert res.shape == o.shape and res.dtype == dtype
+    u = torch.finfo(dtype).eps / 2
+    # half a step of o, and the residual's own rounding
+    assert bool((res.float().abs() <= u * o.float().abs() * (1 + 2 * u) + 1e-7).all())
+    assert float(res.float().abs().max()) > 0 or n * H < 3
+    # the same values, without the outputs' rounding, from float32 inputs: apart
+    # by the probabilities' rounding only
+    seen = window_mask(torch.arange(n).expand(B, n) if pos is None else pos,
+                       torch.zeros(B, dtype=torch.int64), Lk, W, S)
+    ref, tol = bounds(q, k, v, seen, 0.125, dtype)
+    full = (o.double() + res.double()).transpose(1, 2).cpu()
+    assert bool(((full - ref[0]).abs() <= (tol[0] - u * ref[0].abs()) * 1.001
+                 + u * u * ref[0].abs() * 2 + 1e-7).all())
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("Lq", [1, 5, 190])
 def test_rows_without_a_place(dtype, Lq):
@@ -336,8 +364,9 @@ def test_module_calls():
     g = torch.randn(2, 100, 384, generator=gen).to(BF16).to(DEV)
     out.backward(g)
     with torch.no_grad():
-        o, lse = sink_window_attention_fwd(qd, kd, vd, 32, 3, 0.125)
-        want = sink_window_attention_bwd(qd, kd, vd, o, lse, g.view(2, 100, 6, 64), 32, 3, 0.125)
+        o, lse, res = sink_window_attention_fwd(qd, kd, vd, 32, 3, 0.125, return_residual=True)
+        want = sink_window_attention_bwd(qd, kd, vd, o, lse, g.view(2, 100, 6, 64), 32, 3, 0.125,
+                                         o_residual=res)
         assert torch.equal(out, o.view(2, 100, 384)) and torch.equal(layer(qd, kd, vd)[0], out)
     for t, w in zip((qd, kd, vd), want):
         assert torch.equal(t.grad, w)
@@ -346,7 +375,7 @@ def test_module_calls():
     layer(qd, kd, vd)[0].sum().backward()
     ones = torch.ones(2, 100, 6, 64, dtype=BF16, device=DEV)
     assert torch.equal(qd.grad, sink_window_attention_bwd(
-        qd.detach(), kd.detach(), vd.detach(), o, lse, ones, 32, 3, 0.125)[0])
+        qd.detach(), kd.detach(), vd.detach(), o, lse, ones, 32, 3, 0.125, o_residual=res)[0])
     with torch.no_grad():
         assert layer(qd[:, :, :0], kd, vd)[0].shape == (2, 0, 384)
         assert layer(qd[:0], kd[:0], vd[:0])[0].shape == (0, 100, 384)
