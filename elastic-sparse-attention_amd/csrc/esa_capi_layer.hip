@@ -185,17 +185,43 @@ void sink_pattern(SinkArgs& g, const esa_window* w) {
   g.nqb = (g.q_len + 127) / 128;
 }
 
-// Few rows against many keys: the decode kernel (row tiles of 16 over the
-// heads that share a kv head, keys cut into ranges).
-bool sink_decodes(const SinkArgs& g) {
-  return (int64_t)g.groups * g.q_len <= 64 && (int64_t)g.B * g.H * g.q_len < kMaxGrid / 4;
+// Keys that a call's rows walk, at most.
+int64_t sink_keys(const SinkArgs& g) {
+  return std::min<int64_t>(g.kv_len, (int64_t)g.window + g.sinks + g.q_len);
 }
 
+// Few rows against many keys take the decode kernel (row tiles of 16 over the
+// heads that share a kv head, the keys cut into ranges side by side), others
+// the forward's 128-row blocks, which walk their keys one after the other.
+// Both estimated: a block walks a key in 0.022 us (float32: 0.08), blocks past
+// the chip's 512 (256) wait for a round; the decode kernel does 13500 (tile,
+// key) pairs a microsecond at head_dim 128, twice that at 64 (float32: 2500,
+// 5000), after 8 us.  Measured, decode against blocks: bf16, head_dim 128, 32
+// heads on 8, window 4096, one sequence, 1 / 16 / 64 rows 13 / 16 / 36 us
+// against 91 / 92 / 94; 8 sequences, 4 / 16 / 32 rows 33 / 95 / 152 against
+// 108 / 115 / 104; 64 sequences, window 1024, 4 / 8 / 16 / 32 rows 55 / 81 /
+// 154 / 302 against 142 / 143 / 144 / 144; float32, head_dim 64, 64 rows 28
+// against 91.
+bool sink_decodes(const SinkArgs& g) {
+  if ((int64_t)g.B * g.H * g.q_len >= kMaxGrid / 4) return false;
+  const bool f32 = g.elem == ESA_F32;
+  const double keys = (double)sink_keys(g);
+  const double tiles = (double)g.B * g.Hkv * (((int64_t)g.groups * g.q_len + 15) / 16);
+  const int64_t blocks = (int64_t)g.B * g.H * g.nqb, slots = f32 ? 256 : 512;
+  const double rate = (f32 ? 2500.0 : 13500.0) * (g.d_real <= 64 ? 2.0 : 1.0);
+  return tiles * keys / rate + 8.0 < keys * (f32 ? 0.08 : 0.022) * (double)((blocks + slots - 1) / slots)
+         || (int64_t)g.groups * g.q_len <= 16;
+}
+
+// Key ranges a row tile: as many as make 512 workgroups (two a CU: with 1024
+// a 64-sequence step took 191 us against 184, four long sequences 102 against
+// 94), each of at least 128 keys, 32 a wave (one sequence over 1028 keys: 9.9
+// us with 128, 11.3 with 256).
 void sink_splits(SinkArgs& g) {
   g.row_tiles = (g.groups * g.q_len + 15) / 16;
-  const int64_t keys = std::min<int64_t>(g.kv_len, (int64_t)g.window + g.sinks + g.q_len);
+  const int64_t keys = sink_keys(g);
   const int64_t units = (int64_t)g.B * g.Hkv * g.row_tiles;
-  g.splits = (int)std::min<int64_t>((keys + 127) / 128, std::max<int64_t>(1, 1024 / units));
+  g.splits = (int)std::min<int64_t>((keys + 127) / 128, std::max<int64_t>(1, 512 / units));
 }
 
 SinkArgs sink_fwd_args(const esa_fwd_args* a, const esa_window* w) {

@@ -11,7 +11,13 @@
 // the keys were cut, the ranges' in a second kernel.
 //
 // Bound: HBM (every visible key and value is read once); what hides its
-// latency is the number of waves, each with 32 keys' K and V in flight.
+// latency is the number of waves, each with 32 keys' K and V in flight: 64
+// sequences over 4096-key windows of 8 kv heads at head_dim 128, 1.08 GB, in
+// 184 us (5.9 TB/s, the rate of a gather of such rows); 4 sequences over
+// 131072 keys of 2 kv heads, 488 MB, in 94 us with the join.  One sequence is
+// bound by latency: 1028 keys of 8 kv heads in 72 workgroups take 6.9 us and
+// 3.4 the join (one workgroup of 16 waves a kv head and no join took 16.7: a
+// CU alone draws 16 bytes a clock from HBM).
 #include "esa_sink.hpp"
 
 namespace esa {
@@ -308,12 +314,12 @@ __global__ __launch_bounds__(256, 2) void sink_decode_kernel(SinkArgs A) {
   }
 }
 
-// The key ranges of one row, joined in order: 8 groups of lanes take every
-// eighth range, each lane 4 dims (and pass).
+// The key ranges of one row, joined in order: GR groups of lanes take every
+// GR-th range, each lane 4 dims, then the groups' sums in LDS.
 template <int D, Elem E>
-__global__ __launch_bounds__(256) void sink_decode_join_kernel(SinkArgs A) {
+__global__ __launch_bounds__(512) void sink_decode_join_kernel(SinkArgs A) {
   using EL = typename ElemT<E>::T;
-  constexpr int LPR = D / 4, GR = 256 / LPR;
+  constexpr int LPR = D / 4, GR = 512 / LPR;
   __shared__ __attribute__((aligned(16))) float ob[GR][D];
   __shared__ float wsum[GR][2];
   const int n_rows = A.groups * A.q_len;
@@ -382,7 +388,7 @@ hipError_t launch_decode(const SinkArgs& a, hipStream_t stream) {
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
   sink_decode_join_kernel<D, E>
-      <<<(unsigned)((int64_t)a.B * a.H * a.q_len), 256, 0, stream>>>(a);
+      <<<(unsigned)((int64_t)a.B * a.H * a.q_len), 512, 0, stream>>>(a);
   return hipGetLastError();
 }
 
