@@ -13,13 +13,14 @@
 //   dgain = sum over rows of g * n,   dx = r (g gain - n mean(g gain n))
 //
 // Bound: HBM (each row is read and written once; in the backward x and dy are
-// read and dx written).  A workgroup takes a tile of up to eight tokens, forms
-// their cosines and sines once in LDS (one float64 product and one sincospi
-// per pair and token, shared by all heads), then streams the rows of every
-// head: LPR lanes of a wave hold a row, V elements each (16 bytes, or 8 where
-// a pair's halves do not start on 16-byte pieces), and a pair's other half
-// comes from its lane by a shuffle.  Tables of cosines would be read from HBM
-// per token; here nothing but the frequencies is.
+// read and dx written), and next to it the instructions a row takes.  LPR
+// lanes of a wave hold a row, V elements each (16 bytes, or 8 where a pair's
+// halves do not start on 16-byte pieces), and keep to one token: its cosines
+// and sines are formed once in LDS (one float64 product and one sincospi a
+// pair, shared by all heads; tables would be read from HBM) and stay in
+// registers while the lanes go through its heads, the next head's row on its
+// way.  A pair's other half comes from its lane by a DPP rotation (16 lanes a
+// row) or a shuffle.
 #include "esa_rotary.hpp"
 #include "esa_mma.hpp"
 
@@ -82,12 +83,31 @@ __device__ __forceinline__ void store_gain(void* w, int elem, int i, float x) {
     ElemT<Elem::f16>::store((uint16_t*)w + i, x);
 }
 
+// x of the lane that holds the other halves of this lane's pairs
+template <int LPR>
+__device__ __forceinline__ float other_half(float x, int partner, bool across8) {
+  if (LPR == 16 && across8) {
+    // lane l ^ 8: a rotation by 8 in each row of 16 lanes
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(
+        0, (int)__float_as_uint(x), 0x128, 0xf, 0xf, true));
+  }
+  return __shfl(x, partner, 64);
+}
+
+template <int LPR>
+__device__ __forceinline__ float row_sum(float x) {
+#pragma unroll
+  for (int off = LPR / 2; off >= 1; off >>= 1) x += __shfl_xor(x, off, 64);
+  return x;
+}
+
 template <Elem E, int V, int LPR, int MODE>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs A) {
   using T = typename ElemT<E>::T;
-  constexpr int RPP = 256 / LPR;  // rows a pass
-  __shared__ float2 cs[kRotaryTokens * 128];
-  __shared__ int64_t slot[kRotaryTokens];  // append: cache row, or -1
+  using P = Piece<E, V>;
+  using W = decltype(P::w);
+  constexpr int TOK = 256 / LPR;  // tokens of a tile
+  __shared__ float2 cs[TOK * (LPR * V / 2)];
 
   const int tid = threadIdx.x;
   const int lane = tid % LPR, sub = tid / LPR;
@@ -95,12 +115,11 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs A) {
   const bool on = e0 < A.D;
   const int half = A.rd / 2;
   // this lane's part in the rotation: first element's pair, its partner lane
-  // and the sign of the partner's product (pairs of halves)
   const bool rot = e0 < A.rd;
   const bool second = !A.interleaved && e0 >= half;
   const int pair0 = A.interleaved ? e0 / 2 : second ? e0 - half : e0;
   const int partner = (tid & 63) + (rot && !A.interleaved ? (second ? -half / V : half / V) : 0);
-  const float sign = second ? 1.f : -1.f;
+  const bool across8 = half == 8 * V;  // (lanes past rd take the value and multiply it by 0)
 
   float wq[V], wk[V];
 #pragma unroll
@@ -112,24 +131,18 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs A) {
 #pragma unroll
   for (int e = 0; e < V; ++e) gq[e] = gk[e] = 0.f;
 
+  // this workgroup's heads among q's, k's and (append) v's
   const int h0 = blockIdx.y * A.heads_per_split;
-  const int nh = min(A.heads_per_split, A.heads - h0);
+  const int h1 = min(h0 + A.heads_per_split, A.heads);
   const float inv_d = 1.f / (float)A.D;
 
   for (int tile = blockIdx.x; tile < A.n_tiles; tile += gridDim.x) {
-    const int b = (int)fast_div((uint32_t)tile, A.div_tiles);
-    const int t0 = (tile - b * A.tiles_per_seq) << A.log_t;
-    const int nt = min(1 << A.log_t, A.n - t0);
-    const int64_t* pos = A.pos + (int64_t)b * A.pos_sb;
+    const int g0 = tile * TOK, nt = min(TOK, A.tokens - g0);
     if (tile != (int)blockIdx.x) __syncthreads();  // the previous tile's reads of cs
-    int64_t base = 0;
-    if constexpr (MODE == kAppend) {
-      base = pos[0];
-      base += base < 0 ? A.kv_len : 0;
-    }
     for (int i = tid; i < nt * half; i += 256) {
       const int t = (int)fast_div((uint32_t)i, A.div_half), f = i - t * half;
-      int64_t p = pos[t0 + t];
+      const int b = (int)fast_div((uint32_t)(g0 + t), A.div_n);
+      int64_t p = A.pos[(int64_t)b * A.pos_sb + (g0 + t - b * A.n)];
       if constexpr (MODE == kAppend) p += p < 0 ? A.kv_len : 0;
       double turns = (double)p * A.inv_freq[f] * 0.15915494309189533577;
       turns -= rint(turns);
@@ -137,148 +150,116 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs A) {
       sincospif(2.f * (float)turns, &s, &c);
       cs[i] = make_float2(c, s);
     }
+    __syncthreads();
+    if (sub >= nt) continue;  // (no barrier before the next tile's first one)
+
+    const int64_t b = fast_div((uint32_t)(g0 + sub), A.div_n), s = g0 + sub - b * A.n;
+    int64_t os = s;  // the output's row
     if constexpr (MODE == kAppend) {
       // row s of the sequence belongs at base + s inside the cache; any other
       // position (out of range, repeated, out of order) is written nowhere
-      if (tid < nt) {
-        int64_t p = pos[t0 + tid];
-        p += p < 0 ? A.kv_len : 0;
-        slot[tid] = base >= 0 && p == base + t0 + tid && p < A.kv_len ? p : -1;
-      }
+      const int64_t* pos = A.pos + b * A.pos_sb;
+      int64_t base = pos[0], p = pos[s];
+      base += base < 0 ? A.kv_len : 0;
+      p += p < 0 ? A.kv_len : 0;
+      os = base >= 0 && p == base + s && p < A.kv_len ? p : -1;
     }
-    __syncthreads();
-
-    const int rows = nt * nh;
-    for (int row = sub; row < rows; row += RPP) {
-      // heads are the fast axis where a token's heads lie next to each other
-      int t, hh;
-      if (A.heads_fast) {
-        t = (int)fast_div((uint32_t)row, A.div_heads);
-        hh = row - t * nh;
-        if (nh != A.heads_per_split) {  // the last split's shorter rows
-          t = row / nh;
-          hh = row - t * nh;
-        }
-      } else if (nt == 1 << A.log_t) {
-        hh = row >> A.log_t;
-        t = row - (hh << A.log_t);
+    // y[e] = x[e] c[e] + (the pair's other element) sn[e]
+    float c[V], sn[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      float2 t = make_float2(1.f, 0.f);
+      if (rot) t = cs[sub * half + pair0 + (A.interleaved ? e / 2 : e)];
+      c[e] = t.x;
+      sn[e] = (A.interleaved ? e & 1 : second) ? t.y : -t.y;
+    }
+    auto turn = [&](const float (&x)[V], float (&y)[V], float dir) __attribute__((always_inline)) {
+      if (A.interleaved) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) y[e] = x[e] * c[e] + dir * x[e ^ 1] * sn[e];
       } else {
-        hh = row / nt;
-        t = row - hh * nt;
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          y[e] = x[e] * c[e] + dir * other_half<LPR>(x[e], partner, across8) * sn[e];
       }
-      hh += h0;
-      const int64_t s = t0 + t;
-      int64_t os = s;  // the output's row
-      if constexpr (MODE == kAppend) os = slot[t];
-      const int kind = hh < A.H ? 0 : hh < A.H + A.Hkv ? 1 : 2;
-      const int h = kind == 0 ? hh : hh - A.H - (kind == 2 ? A.Hkv : 0);
-
-      const T* src = kind == 0 ? (const T*)A.q + b * A.qsb + h * A.qsh + s * A.qss
-                   : kind == 1 ? (const T*)A.k + b * A.ksb + h * A.ksh + s * A.kss
-                               : (const T*)A.v + b * A.vsb + h * A.vsh + s * A.vss;
-      Piece<E, V> in;
-      in.w = decltype(in.w){};
-      if (on) in.w = *(const decltype(in.w)*)(src + e0);
-      if constexpr (MODE == kAppend) {
-        if (kind == 2) {  // values go to their cache as they are
-          if (on && os >= 0)
-            *(decltype(in.w)*)((T*)A.vo + b * A.vosb + h * A.vosh + os * A.voss + e0) = in.w;
-          continue;
+      // (elements past rotary_dim as they are: a neighbour's infinity is not theirs)
+#pragma unroll
+      for (int e = 0; e < V; ++e) y[e] = rot ? y[e] : x[e];
+    };
+    // `count` heads of q or k from src (and g), results to dst (or nowhere)
+    auto heads = [&](const T* src, int64_t sh, const T* g, int64_t gh, T* dst, int64_t dh,
+                     int count, const float (&w)[V], float (&sums)[V], bool lost)
+                     __attribute__((always_inline)) {
+      P in, gin;
+      in.w = gin.w = W{};
+      if (on) in.w = *(const W*)src;
+      if (MODE == kBwd && on) gin.w = *(const W*)g;
+      for (int i = 0; i < count; ++i) {
+        const P xin = in, ggin = gin;
+        src += sh;
+        g += gh;
+        if (i + 1 < count && on) {  // the next head's row, on its way meanwhile
+          in.w = *(const W*)src;
+          if (MODE == kBwd) gin.w = *(const W*)g;
         }
-      }
-      float x[V], ss = 0.f;
+        float x[V], y[V], ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        x[e] = in.get(e);
-        ss = __builtin_fmaf(x[e], x[e], ss);
-      }
-      const float2* crow = cs + t * half;
-
-      if constexpr (MODE != kBwd) {
-#pragma unroll
-        for (int off = LPR / 2; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, 64);
-        const float r = 1.f / sqrtf(__builtin_fmaf(ss, inv_d, A.eps));
-        float y[V];
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[e] *= r * (kind == 0 ? wq[e] : wk[e]);
-        if (A.interleaved) {
-#pragma unroll
-          for (int e = 0; e < V; e += 2) {
-            const float2 c = rot ? crow[pair0 + e / 2] : make_float2(1.f, 0.f);
-            y[e] = x[e] * c.x - x[e + 1] * c.y;
-            y[e + 1] = x[e + 1] * c.x + x[e] * c.y;
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float2 c = rot ? crow[pair0 + e] : make_float2(1.f, 0.f);
-            y[e] = x[e] * c.x + sign * __shfl(x[e], partner, 64) * c.y;
-          }
+        for (int e = 0; e < V; ++e) {
+          x[e] = xin.get(e);
+          ss = __builtin_fmaf(x[e], x[e], ss);
         }
-        if constexpr (MODE == kAppend) {
-          if (os < 0) {
-            if (kind == 1) continue;
-            // a query row with no place in the cache: NaN, as the attention
-            // over the cache gives it
+        if constexpr (MODE != kBwd) {
+          const float r = rsqrtf(__builtin_fmaf(row_sum<LPR>(ss), inv_d, A.eps));
+#pragma unroll
+          for (int e = 0; e < V; ++e) x[e] *= r * w[e];
+          turn(x, y, 1.f);
+          if (MODE == kAppend && lost) {
 #pragma unroll
             for (int e = 0; e < V; ++e) y[e] = __builtin_nanf("");
-            os = s;
-          }
-          if (kind == 0) os = s;
-        }
-        if (on) {
-          T* dst = kind == 0 ? (T*)A.qo + b * A.qosb + h * A.qosh + os * A.qoss
-                             : (T*)A.ko + b * A.kosb + h * A.kosh + os * A.koss;
-          store_piece<E, V>(dst + e0, y);
-        }
-      } else {
-        const T* gsrc = kind == 0 ? (const T*)A.gq + b * A.gqsb + h * A.gqsh + s * A.gqss
-                                  : (const T*)A.gk + b * A.gksb + h * A.gksh + s * A.gkss;
-        Piece<E, V> gin;
-        gin.w = decltype(gin.w){};
-        if (on) gin.w = *(const decltype(gin.w)*)(gsrc + e0);
-        float g[V], y[V], dot = 0.f;
-#pragma unroll
-        for (int e = 0; e < V; ++e) g[e] = gin.get(e);
-        // the rotation undone
-        if (A.interleaved) {
-#pragma unroll
-          for (int e = 0; e < V; e += 2) {
-            const float2 c = rot ? crow[pair0 + e / 2] : make_float2(1.f, 0.f);
-            y[e] = g[e] * c.x + g[e + 1] * c.y;
-            y[e + 1] = g[e + 1] * c.x - g[e] * c.y;
           }
         } else {
+          float gr[V], dot = 0.f;
+#pragma unroll
+          for (int e = 0; e < V; ++e) gr[e] = ggin.get(e);
+          turn(gr, y, -1.f);  // the rotation undone
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            const float2 c = rot ? crow[pair0 + e] : make_float2(1.f, 0.f);
-            y[e] = g[e] * c.x - sign * __shfl(g[e], partner, 64) * c.y;
+            gr[e] = y[e] * w[e];
+            dot = __builtin_fmaf(gr[e], x[e], dot);
+          }
+          ss = row_sum<LPR>(ss);
+          dot = row_sum<LPR>(dot);
+          const float r = rsqrtf(__builtin_fmaf(ss, inv_d, A.eps));
+          const float m = dot * inv_d * r * r;  // mean(g gain n) r
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            sums[e] += y[e] * (x[e] * r);
+            y[e] = r * (gr[e] - x[e] * m);
           }
         }
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          g[e] = y[e] * (kind == 0 ? wq[e] : wk[e]);
-          dot = __builtin_fmaf(g[e], x[e], dot);
-        }
-#pragma unroll
-        for (int off = LPR / 2; off >= 1; off >>= 1) {
-          ss += __shfl_xor(ss, off, 64);
-          dot += __shfl_xor(dot, off, 64);
-        }
-        const float r = 1.f / sqrtf(__builtin_fmaf(ss, inv_d, A.eps));
-        const float m = dot * inv_d * r * r;  // mean(g gain n) r
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float gn = y[e] * (x[e] * r);
-          if (kind == 0) gq[e] += gn; else gk[e] += gn;
-          g[e] = r * (g[e] - x[e] * m);
-        }
-        if (on) {
-          T* dst = kind == 0 ? (T*)A.qo + b * A.qosb + h * A.qosh + s * A.qoss
-                             : (T*)A.ko + b * A.kosb + h * A.kosh + s * A.koss;
-          store_piece<E, V>(dst + e0, g);
-        }
+        if (on) store_piece<E, V>(dst, y);
+        dst += dh;
       }
+    };
+    const int nq = min(h1, A.H) - h0;
+    if (nq > 0)
+      heads((const T*)A.q + b * A.qsb + h0 * A.qsh + s * A.qss + e0, A.qsh,
+            (const T*)A.gq + b * A.gqsb + h0 * A.gqsh + s * A.gqss + e0, A.gqsh,
+            (T*)A.qo + b * A.qosb + h0 * A.qosh + s * A.qoss + e0, A.qosh, nq, wq, gq,
+            // a query row with no place in the cache: NaN, as the attention
+            // over the cache gives it
+            MODE == kAppend && os < 0);
+    const int k0 = max(h0 - A.H, 0), nk = min(h1 - A.H, A.Hkv) - k0;
+    if (nk > 0 && os >= 0)
+      heads((const T*)A.k + b * A.ksb + k0 * A.ksh + s * A.kss + e0, A.ksh,
+            (const T*)A.gk + b * A.gksb + k0 * A.gksh + s * A.gkss + e0, A.gksh,
+            (T*)A.ko + b * A.kosb + k0 * A.kosh + os * A.koss + e0, A.kosh, nk, wk, gk, false);
+    if constexpr (MODE == kAppend) {  // values go to their cache as they are
+      const int v0 = max(h0 - A.H - A.Hkv, 0), v1 = h1 - A.H - A.Hkv;
+      const T* src = (const T*)A.v + b * A.vsb + v0 * A.vsh + s * A.vss + e0;
+      T* dst = (T*)A.vo + b * A.vosb + v0 * A.vosh + os * A.voss + e0;
+      for (int h = v0; h < v1 && os >= 0 && on; ++h, src += A.vsh, dst += A.vosh)
+        *(W*)dst = *(const W*)src;
     }
   }
 
@@ -295,7 +276,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs A) {
       __syncthreads();
       for (int d = tid; d < A.D; d += 256) {
         float sum = 0.f;
-        for (int i = 0; i < RPP; ++i) sum += red[i * (LPR * V) + d];
+        for (int i = 0; i < TOK; ++i) sum += red[i * (LPR * V) + d];
         out[which * A.D + d] = sum;
       }
     }
@@ -327,12 +308,11 @@ __global__ __launch_bounds__(1024) void rotary_gain_kernel(const float* partial,
 
 template <Elem E, int V, int MODE>
 void launch_lpr(const RotaryArgs& a, dim3 grid, hipStream_t stream) {
-  const int lanes = (a.D + V - 1) / V;
-  if (lanes <= 8)
+  if (a.lanes == 8)
     rotary_kernel<E, V, 8, MODE><<<grid, 256, 0, stream>>>(a);
-  else if (lanes <= 16)
+  else if (a.lanes == 16)
     rotary_kernel<E, V, 16, MODE><<<grid, 256, 0, stream>>>(a);
-  else if (lanes <= 32)
+  else if (a.lanes == 32)
     rotary_kernel<E, V, 32, MODE><<<grid, 256, 0, stream>>>(a);
   else
     rotary_kernel<E, V, 64, MODE><<<grid, 256, 0, stream>>>(a);

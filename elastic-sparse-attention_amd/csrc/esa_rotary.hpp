@@ -4,8 +4,6 @@
 
 namespace esa {
 
-constexpr int kRotaryTokens = 8;  // tokens of a tile, at most
-
 struct RotaryArgs {
   const void *q, *k, *v;  // rows in (v: append only)
   void *qo, *ko, *vo;     // rows out: q, k; append: q and the two caches; backward: dq, dk
@@ -22,11 +20,11 @@ struct RotaryArgs {
   int elem, welem, vec;  // vec: elements a lane holds
   int interleaved;
   float eps;
-  // the grid: tiles of 2^log_t tokens of one sequence, heads (q, k and, to
-  // append, v) in splits; grid_tiles workgroups walk the n_tiles tiles
-  int log_t, tiles_per_seq, n_tiles, grid_tiles;
-  int heads, heads_per_split, n_splits, heads_fast;
-  FastDiv div_tiles, div_half, div_heads;
+  // the grid: tiles of 256 / (lanes a row) of all sequences' tokens, heads (q, k
+  // and, to append, v) in splits; grid_tiles workgroups walk the n_tiles tiles
+  int lanes, tokens, n_tiles, grid_tiles;
+  int heads, heads_per_split, n_splits;
+  FastDiv div_n, div_half;
   float* partial;  // backward: [grid_tiles n_splits][2][D] sums of the gains' gradients
 };
 

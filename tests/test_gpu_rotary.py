@@ -197,6 +197,25 @@ def test_special_rows():
     assert torch.equal(~torch.isfinite(y).all(-1), bad)
 
 
+@pytest.mark.parametrize("inter", [False, True])
+def test_elements_past_the_rotation_are_their_own(inter):
+    # an infinite gain or gradient reaches its own element (and its pair's),
+    # no neighbour's
+    D, rd = 64, 32
+    q, k, wq, wk, pos, freq, gen = case(1, 2, 1, 3, D, rd, F32, "bhld")
+    wq[40] = float("inf")
+    yq, _ = qk_norm_rope_fwd(q.to(DEV), k.to(DEV), wq.to(DEV), wk.to(DEV), freq.to(DEV),
+                             pos.to(DEV), 1e-6, inter)
+    finite = torch.isfinite(yq.cpu())
+    assert not finite[..., 40].any() and int((~finite).sum()) == yq[..., 40].numel()
+    gq, gk = torch.randn(q.shape, generator=gen), torch.randn(k.shape, generator=gen)
+    gq[0, 0, 1, 50] = float("inf")
+    _, _, dwq, _ = qk_norm_rope_bwd(q.to(DEV), k.to(DEV), wk.to(DEV), wk.to(DEV), freq.to(DEV),
+                                    pos.to(DEV), gq.to(DEV), gk.to(DEV), 1e-6, inter)
+    finite = torch.isfinite(dwq.cpu())
+    assert not finite[50] and int((~finite).sum()) == 1
+
+
 @pytest.mark.parametrize("dtype,D,rd,inter", [(BF16, 128, 128, False), (F16, 64, 32, True),
                                               (F32, 80, 80, False), (BF16, 72, 72, False)])
 @pytest.mark.parametrize("n", [1, 5, 150])
