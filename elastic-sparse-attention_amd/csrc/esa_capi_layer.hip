@@ -257,10 +257,11 @@ int sink_qpad(int q_len) { return (q_len + 3) / 4 * 4; }
 // do and about `part` stages more for its float32 part (written, read and
 // joined).  Counted so, with the blocks alike (a window):
 //   a sinks' block is cut into pieces of a window block's size;
-//   of U blocks the whole rounds stay whole, and the U mod slots that would
-//   fill a last round by themselves are cut so that they fill it together
-//   (8192 rows, 8 kv heads of 4 query heads, window 1024, head_dim 128: 568
-//   blocks on 512 slots, two rounds of 76 stages against one and a ninth);
+//   of all blocks the whole rounds stay whole, and those that would run as an
+//   unfilled last round (or all of a grid too small for one) are cut so that
+//   they fill it together (8192 rows, 8 kv heads of 4 query heads, window 1024
+//   and 4 sinks, head_dim 128: 568 blocks on 512 slots, two rounds of 72 stages
+//   against one and a fifth: 480 us, 365);
 // where the first blocks see many more rows than the last (a window near the
 // sequence's length) all are cut alike, to at most 2/3 of a slot's share.
 void sink_bwd_plan(SinkArgs& g) {
@@ -275,50 +276,48 @@ void sink_bwd_plan(SinkArgs& g) {
   const int64_t n_reg = g.nkb - n_sink;
   const int64_t span = std::min<int64_t>(g.window + 127, g.q_len);
   const double mean = 1.0 - 0.5 * (double)span / (double)std::max<int64_t>(g.q_len, 1);
-  int cut[2] = {1, 1};
-  int64_t n_last = 0;
-  auto best_cut = [&](int64_t blocks, int64_t whole_rounds) {
-    int64_t best = 0;
-    int c_best = 1;
-    for (int c = 1; c <= 16 && c <= one; ++c) {
-      const int64_t rounds = (blocks * c + slots - 1) / slots;
-      const int64_t cost = whole_rounds * one + rounds * ((one + c - 1) / c + (c > 1 ? part : 0));
-      if (c == 1 || cost < best) {
-        best = cost;
-        c_best = c;
-      }
-    }
-    return c_best;
-  };
-  if (n_reg > 0) {
-    if (mean < 0.75) {
-      const double share = (double)kv * n_reg * one * mean / (double)slots;
-      cut[0] = cut[1] = (int)std::max(1.0, std::min(8.0, std::ceil(1.5 * one / share)));
-      cut[0] = cut[1] = (int)std::max<int64_t>(1, std::min<int64_t>(cut[0], 4 * slots / (kv * n_reg)));
-    } else {
-      const int64_t blocks = kv * n_reg, over = blocks % slots;
-      if (blocks < slots) {
-        cut[0] = cut[1] = best_cut(blocks, 0);
-      } else if (over > 0 && blocks < 8 * slots) {
-        cut[1] = best_cut(over, blocks / slots);
-        n_last = cut[1] > 1 ? (over + kv - 1) / kv : 0;
-      }
-    }
+  const bool alike = mean >= 0.75;
+  int64_t cut = 1, n_last = 0, cut_last = 1;
+  if (!alike && n_reg > 0) {
+    const double share = (double)kv * n_reg * one * mean / (double)slots;
+    cut = (int64_t)std::max(1.0, std::min(8.0, std::ceil(1.5 * one / share)));
+    cut = std::max<int64_t>(1, std::min<int64_t>(cut, 4 * slots / (kv * n_reg)));
   }
-  // the sinks' pieces as long as the shortest chunk of the others, within
-  // 256 MiB of parts
+  // the sinks' pieces as long as the others' chunks, within 256 MiB of parts
   int64_t sink_cut = 1;
   if (n_sink > 0) {
-    const int64_t piece = std::max<int64_t>(1, one / std::max(1, cut[0]));
+    const int64_t piece = std::max<int64_t>(1, one / cut);
     sink_cut = std::min<int64_t>(64, (stages(g.q_len) + piece - 1) / piece);
     sink_cut = std::min(sink_cut, std::max<int64_t>(1, 2048 / (kv * n_sink)));
   }
+  const int64_t pieces = kv * n_sink * sink_cut, total = pieces + kv * n_reg;
+  if (alike && n_reg > 0 && total % slots != 0 && total < 8 * slots) {
+    // the time, in stages, of `whole` blocks and then `chunks` chunks of `size`,
+    // each taken by the next free slot
+    auto time = [&](int64_t whole, int64_t chunks, int64_t size) {
+      const int64_t rounds = whole / slots, rem = whole % slots;
+      int64_t k = 0;  // chunks a slot that was free after `rounds`
+      while ((slots - rem) * k + rem * std::max<int64_t>(0, (k * size - one) / size) < chunks) ++k;
+      return std::max(rounds * one + k * size, (rounds + (rem > 0)) * one);
+    };
+    int64_t best = time(total, 0, one);
+    const int64_t over = std::min<int64_t>(n_reg, (total % slots + kv - 1) / kv);
+    for (const int64_t n : {over, n_reg})
+      for (int64_t c = 2; c <= 16 && c <= one && kv * n * c <= 4 * slots; ++c) {
+        const int64_t t = time(total - kv * n, kv * n * c, (one + c - 1) / c + part);
+        if (t < best) {
+          best = t;
+          n_last = n;
+          cut_last = c;
+        }
+      }
+  }
   g.cls_n[0] = n_sink;
   g.cls_cut[0] = (int)sink_cut;
-  g.cls_n[2] = (int)std::min<int64_t>(n_last, n_reg);
-  g.cls_n[1] = (int)n_reg - g.cls_n[2];
-  g.cls_cut[1] = cut[0];
-  g.cls_cut[2] = cut[1];
+  g.cls_n[1] = (int)(n_reg - n_last);
+  g.cls_cut[1] = (int)cut;
+  g.cls_n[2] = (int)n_last;
+  g.cls_cut[2] = (int)cut_last;
 }
 
 struct SinkBwdSizes {
