@@ -226,6 +226,16 @@ struct SinkTile {
       f.f[s] = __builtin_bit_cast(V8, raw);
     }
   }
+  // c + the lane's share (its half of the dims) of the product of two rows
+  static __device__ __forceinline__ float dot(const Frag& a, const Frag& b, float c) {
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        c = __builtin_fmaf(ElemT<E>::chunk(__builtin_bit_cast(u32x4, a.f[s]), e),
+                           ElemT<E>::chunk(__builtin_bit_cast(u32x4, b.f[s]), e), c);
+    return c;
+  }
   __device__ __forceinline__ void row_product(f32x16& acc, const LdsT* buf, int rb,
                                               const Frag& f) const {
     V8 a[NS];
@@ -330,6 +340,13 @@ struct SinkTile<D, Elem::f32, TIGHT> {
       if (ok && d < d_real) raw = *(const f32x4*)((const float*)row + d);
       f.f[u] = raw;
     }
+  }
+  static __device__ __forceinline__ float dot(const Frag& a, const Frag& b, float c) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) c = __builtin_fmaf(a.f[u][t], b.f[u][t], c);
+    return c;
   }
   __device__ __forceinline__ void row_product(f32x16& acc, const float* buf, int rb,
                                               const Frag& f) const {
