@@ -182,7 +182,7 @@ __device__ __forceinline__ KeyStages key_stages(const SinkArgs& A, const SeqInfo
 // row, so that both kinds of read meet each bank once.
 // TIGHT: a kernel short of registers forms a read's address from one base with
 // an exclusive or (the chunk's bits, which the swizzle and the read's place
-// share) each time, instead of keeping one register a read.
+// share) for each product anew, instead of keeping one register a read.
 template <int D, Elem E, bool TIGHT = false>
 struct SinkTile {
   using M = MmaT<E>;
@@ -200,7 +200,7 @@ struct SinkTile {
   using LdsT = uint16_t;
   static constexpr uint32_t kOne = E == Elem::bf16 ? 0x3F80u : 0x3C00u;
 
-  int ra[TIGHT ? 1 : NS];  // element offsets of a 32-row block's row reads
+  int ra[TIGHT ? 1 : NS];  // byte offsets of a 32-row block's row reads
   int ca[TIGHT ? 1 : ND];  // ... of its column reads, rows 4 hf + 0 .. 3 (+ 16 u)
   int hf;
 
@@ -209,12 +209,12 @@ struct SinkTile {
     hf = lane >> 5;
     const int l32 = lane & 31, g4 = lane >> 4, lam = lane & 15;
 #pragma unroll
-    for (int s = 0; s < (TIGHT ? 1 : NS); ++s) ra[s] = l32 * D + 8 * ((2 * s + hf) ^ swz(l32));
+    for (int s = 0; s < (TIGHT ? 1 : NS); ++s) ra[s] = 2 * (l32 * D + 8 * ((2 * s + hf) ^ swz(l32)));
     const int row = 4 * hf + (lam >> 2);
 #pragma unroll
     for (int d = 0; d < (TIGHT ? 1 : ND); ++d) {
       const int col = 32 * d + 16 * (g4 & 1) + 4 * (lam & 3);
-      ca[d] = row * D + 8 * ((col >> 3) ^ swz(row)) + (col & 7);
+      ca[d] = 2 * (row * D + 8 * ((col >> 3) ^ swz(row)) + (col & 7));
     }
   }
   __device__ __forceinline__ void load_frag(Frag& f, const void* row, bool ok, int d_real) const {
@@ -244,15 +244,18 @@ struct SinkTile {
 #pragma unroll
     for (int s = 0; s < NS; ++s) acc = M::mfma32(a[s], f.f[s], acc);
   }
-  // element offset `x` of a base, formed where it is used (the empty asm keeps
-  // the compiler from forming all of them ahead and keeping them)
-  static __device__ __forceinline__ int offset(int base, int x) {
+  // A base that the compiler takes for a new value (what a tight kernel's reads
+  // of one product are formed from, so none is kept for the next)
+  static __device__ __forceinline__ int fresh(int base) {
     if constexpr (TIGHT) asm volatile("" : "+v"(base));
-    return base ^ x;
+    return base;
+  }
+  __device__ __forceinline__ V8 row_operand(const LdsT* buf, int rb, int s, int base) const {
+    const int at = TIGHT ? base ^ (32 * s) : ra[s];
+    return *(const V8*)((const char*)buf + at + 64 * rb * D);
   }
   __device__ __forceinline__ V8 row_operand(const LdsT* buf, int rb, int s) const {
-    const int at = TIGHT ? offset(ra[0], 16 * s) : ra[s];
-    return *(const V8*)(buf + at + 32 * rb * D);
+    return row_operand(buf, rb, s, ra[0]);
   }
   // one product of col_product: rows 16 u .. of the block
   static __device__ __forceinline__ void col_step(f32x16& acc, const u32x4& a, const P& p, int u) {
@@ -267,9 +270,13 @@ struct SinkTile {
   }
   // the A operand of dims 32 d .. and rows 16 u .. of block rb, by columns
   __device__ __forceinline__ u32x4 col_operand(const LdsT* buf, int rb, int d, int u) const {
-    const int at = TIGHT ? offset(ca[0], 32 * d) : ca[d];
-    const LdsT* p1 = buf + at + (32 * rb + 16 * u) * D;
-    const LdsT* p2 = buf + (at ^ 16) + (32 * rb + 16 * u + 8) * D;
+    return col_operand(buf, rb, d, u, ca[0]);
+  }
+  __device__ __forceinline__ u32x4 col_operand(const LdsT* buf, int rb, int d, int u,
+                                               int base) const {
+    const int at = TIGHT ? base ^ (64 * d) : ca[d];
+    const char* p1 = (const char*)buf + at + 2 * (32 * rb + 16 * u) * D;
+    const char* p2 = (const char*)buf + (at ^ 32) + 2 * (32 * rb + 16 * u + 8) * D;
     const s16x4 v[2] = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p1),
                         __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p2)};
     return __builtin_bit_cast(u32x4, v);
@@ -395,8 +402,11 @@ struct SinkStage {
   using T = SinkTile<D, E>;
   static constexpr int LOADS = ROWS * T::CPR / THREADS;
   static constexpr int BYTES = ROWS * D * T::ES;
+  // rows of one round of loads: a multiple of the swizzle's period, so a lane's
+  // rounds differ by a scalar alone
+  static constexpr int ROUND = THREADS / T::CPR;
   static_assert(LOADS >= 1 && LOADS * THREADS == ROWS * T::CPR, "whole stage per load round");
-  int off[LOADS];
+  int off;
   __amdgpu_buffer_rsrc_t rs;
   const char* base;
   int64_t stride;  // bytes
@@ -412,13 +422,8 @@ struct SinkStage {
     row_bytes = d_real * T::ES;
     org = 0;
     reach = 0;
-    const int lane = tid & 63, wave = tid >> 6;
-#pragma unroll
-    for (int j = 0; j < LOADS; ++j) {
-      const int slot = (LOADS * wave + j) * 64 + lane;
-      const int row = slot / T::CPR, chunk = (slot % T::CPR) ^ T::swz(row);
-      off[j] = 16 * chunk < row_bytes ? (int)(row * stride) + 16 * chunk : 0x7ffffff0;
-    }
+    const int row = tid / T::CPR, chunk = (tid % T::CPR) ^ T::swz(row);
+    off = 16 * chunk < row_bytes ? (int)(row * stride) + 16 * chunk : 0x7ffffff0;
     // (0x7ffffff0 plus a stage's offset, below 2^30, is past every resource as
     // an unsigned number)
   }
@@ -441,7 +446,8 @@ struct SinkStage {
     const int soff = (row0 - org) * (int)stride;
 #pragma unroll
     for (int j = 0; j < LOADS; ++j)
-      load_lds16(rs, (uint16_t*)dst + (LOADS * wave + j) * 512, off[j], soff);
+      load_lds16(rs, (uint16_t*)dst + (wave + j * (THREADS / 64)) * 512, off,
+                 soff + j * ROUND * (int)stride);
   }
 };
 

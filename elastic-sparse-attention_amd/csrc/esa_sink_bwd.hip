@@ -36,8 +36,11 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D, Elem E>
 struct SinkBwdCfg {
-  static constexpr int STAGE = E == Elem::f32 ? 32 : 64;  // keys (dQ) or rows (dK / dV)
-  static constexpr int NB = STAGE / 32;
+  // dK / dV: where K, V, their gradients and the products would take more than
+  // the 256 registers of a wave in a pair (head_dim 128, 16-bit), V's rows are
+  // kept in LDS, and stages are 32 rows, so that two workgroups' still fit
+  static constexpr bool V_LDS = E != Elem::f32 && D >= 128;
+  static constexpr int ROWS = E == Elem::f32 || V_LDS ? 32 : 64;
   static constexpr int WAVES_PER_SIMD = E == Elem::f32 ? 1 : 2;
 };
 
@@ -88,21 +91,25 @@ __device__ void fix_dq_row(const SinkArgs& A, int b, int h, int kvh, int row, in
 template <int D, Elem E>
 __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_dq_kernel(
     SinkArgs A) {
-  using C = SinkBwdCfg<D, E>;
   using T = SinkTile<D, E>;
-  using Stage = SinkStage<D, E, C::STAGE, 256>;
+  using Stage = SinkStage<D, E, 32, 256>;
   using LdsT = typename T::LdsT;
-  constexpr int ND = T::ND;
-  __shared__ __attribute__((aligned(1024))) LdsT k_st0[C::STAGE * D];
-  __shared__ __attribute__((aligned(1024))) LdsT v_st0[C::STAGE * D];
-  __shared__ __attribute__((aligned(1024))) LdsT k_st1[C::STAGE * D];
-  __shared__ __attribute__((aligned(1024))) LdsT v_st1[C::STAGE * D];
+  constexpr int ND = T::ND, N = 32 * D;
+  // four stages of 32 keys, as the forward's
+  __shared__ __attribute__((aligned(1024))) LdsT k0_[N];
+  __shared__ __attribute__((aligned(1024))) LdsT v0_[N];
+  __shared__ __attribute__((aligned(1024))) LdsT k1_[N];
+  __shared__ __attribute__((aligned(1024))) LdsT v1_[N];
+  __shared__ __attribute__((aligned(1024))) LdsT k2_[N];
+  __shared__ __attribute__((aligned(1024))) LdsT v2_[N];
+  __shared__ __attribute__((aligned(1024))) LdsT k3_[N];
+  __shared__ __attribute__((aligned(1024))) LdsT v3_[N];
 
   const RowItem it = row_item(A);
   const int b = it.b, h = it.h, kvh = it.kvh, r0 = it.qb * 128;
   const SeqInfo si = seq_info(A, b);
   const int f = si.first, sink_end = min(f + A.sinks, A.kv_len), W = A.window;
-  const KeyStages keys = key_stages<C::STAGE>(A, si, r0, sink_end);
+  const KeyStages keys = key_stages<32>(A, si, r0, sink_end);
 
   const int tid = threadIdx.x;
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -111,6 +118,18 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
   const bool row_in = r < A.q_len;
   const int p = si.base + r;
   const int pb = keys.pb, pw0 = si.base + r0 + wave * 32, pw1 = min(pw0 + 31, pb);
+  const int n_all = keys.n_all;
+  const WaveStages ws = wave_stages<32>(keys, pw0, pw1, W, sink_end);
+
+  Stage ks, vs;
+  ks.init(at<E>(A.k, (int64_t)b * A.ksb + (int64_t)kvh * A.ksh), A.kss, A.kv_len, A.d_real, tid);
+  vs.init(at<E>(A.v, (int64_t)b * A.vsb + (int64_t)kvh * A.vsh), A.vss, A.kv_len, A.d_real, tid);
+  auto issue = [&](int i, LdsT* kd, LdsT* vd) __attribute__((always_inline)) {
+    if (i < n_all) {
+      ks.issue(keys.key0(i), kd, wave);
+      vs.issue(keys.key0(i), vd, wave);
+    }
+  };
 
   T t;
   t.init(lane);
@@ -141,47 +160,130 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
   for (int d = 0; d < ND; ++d) acc[d] = f32x16{};
   const float scale = A.scale_log2;
 
-  Stage ks, vs;
-  ks.init(at<E>(A.k, (int64_t)b * A.ksb + (int64_t)kvh * A.ksh), A.kss, A.kv_len, A.d_real, tid);
-  vs.init(at<E>(A.v, (int64_t)b * A.vsb + (int64_t)kvh * A.vsh), A.vss, A.kv_len, A.d_real, tid);
-
-  auto block = [&](const LdsT* kbuf, const LdsT* vbuf, int kb, int k0)
-                   __attribute__((always_inline)) {
-    if (pw0 > pb || none_seen(pw0, pw1, k0, W, sink_end)) return;
-    f32x16 s = f32x16{}, dp = f32x16{};
-    if (!all_seen(pw0, pw0 + 31, k0, W, sink_end))
-      mask_init<0>(s, ~(seen_keys(p, k0, W, sink_end) >> (4 * hf)));
-    t.row_product(s, kbuf, kb, qf);
-    t.row_product(dp, vbuf, kb, gf);
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -lse2)) * (dp[i] - delta);
-    t.col_product(acc, kbuf, kb, t.pack(s));
+  // A pipeline over the stages: s holds the coming stage's scores (of the keys
+  // that the wave sees); its exponentials run beside the product dP, dS beside
+  // the next stage's scores, dQ's product last.
+  f32x16 s = f32x16{};
+  bool used = false;
+  auto hide = [&](f32x16& x, int i) __attribute__((always_inline)) {
+    if (!ws.full(i)) {
+      uint32_t m[16];
+      key_masks<0>(m, seen_keys(p, keys.key0(i), W, sink_end) >> (4 * hf));
+      mask_select(x, m);
+    }
   };
-  auto stage = [&](const LdsT* kbuf, const LdsT* vbuf, int i) __attribute__((always_inline)) {
-    const int k0 = keys.key0(i);
+  // stage i: its K and V, the next stage's K
+  auto step = [&](const LdsT* kbuf, const LdsT* vbuf, const LdsT* knext, int i)
+                  __attribute__((always_inline)) {
+    const bool next = ws.sees(i + 1);
+    if (!used) {
+      if (next) {
+        s = f32x16{};
+        t.row_product(s, knext, 0, qf);
+        hide(s, i + 1);
+      }
+      used = next;
+      return;
+    }
+    f32x16 sn = f32x16{}, dp = f32x16{};
+    if constexpr (T::ES == 2) {
+      // in written order, operands read AHEAD products ahead
+      constexpr int AHEAD = 4, NS = T::NS, PER = 8 / NS;  // PER: pairs of keys a product
+      typename T::V8 va[NS], ka[NS];
+      u32x4 kc[NS];
+      typename T::P pd;
+      auto read = [&](int i) __attribute__((always_inline)) {
+        const int k = i % NS;
+        if (i < NS)
+          va[k] = t.row_operand(vbuf, 0, k);
+        else if (i < 2 * NS)
+          ka[k] = t.row_operand(knext, 0, k);
+        else if (i < 3 * NS)
+          kc[k] = t.col_operand(kbuf, 0, k % ND, k / ND);
+      };
+      auto grads = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
-    for (int kb = 0; kb < C::NB; ++kb) block(kbuf, vbuf, kb, k0 + 32 * kb);
+        for (int q = k * PER; q < (k + 1) * PER; ++q) {
+#pragma unroll
+          for (int e = 2 * q; e < 2 * q + 2; ++e) s[e] *= dp[e] - delta;
+          pd.w[q] = T::M::pack2(s[2 * q], s[2 * q + 1]);
+        }
+      };
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) read(k);
+#pragma unroll
+      for (int k = 0; k < NS; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        dp = T::M::mfma32(va[k], gf.f[k], dp);
+        read(k + AHEAD);
+#pragma unroll
+        for (int e = 2 * k * PER; e < 2 * (k + 1) * PER; ++e)
+          s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], scale, -lse2));
+      }
+      // (past the wave's last key: of whatever the buffer holds, and dropped)
+#pragma unroll
+      for (int k = 0; k < NS; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        sn = T::M::mfma32(ka[k], qf.f[k], sn);
+        read(NS + k + AHEAD);
+        if (k > 0) grads(k - 1);
+      }
+#pragma unroll
+      for (int k = 0; k < NS; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (k == 0) grads(NS - 1);
+        T::col_step(acc[k % ND], kc[k], pd, k / ND);
+        read(2 * NS + k + AHEAD);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    } else {
+      t.row_product(dp, vbuf, 0, gf);
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], scale, -lse2)) * (dp[e] - delta);
+      t.row_product(sn, knext, 0, qf);
+      t.col_product(acc, kbuf, 0, t.pack(s));
+    }
+    if (next) hide(sn, i + 1);
+    s = sn;
+    used = next;
   };
-  const int n_all = keys.n_all;
+  auto ready = [&](int i) __attribute__((always_inline)) {
+    if (i + 2 < n_all)
+      stage_wait<2 * Stage::LOADS>();
+    else
+      stage_wait<0>();
+  };
+  issue(0, k0_, v0_);
+  issue(1, k1_, v1_);
+  issue(2, k2_, v2_);
   if (n_all > 0) {
-    ks.issue(keys.key0(0), k_st0, wave);
-    vs.issue(keys.key0(0), v_st0, wave);
+    if (n_all > 2)
+      stage_wait<4 * Stage::LOADS>();
+    else
+      stage_wait<0>();
+    if (ws.sees(0)) {
+      t.row_product(s, k0_, 0, qf);
+      hide(s, 0);
+      used = true;
+    }
   }
-  for (int i = 0; i < n_all; i += 2) {
-    stage_ready();
-    if (i + 1 < n_all) {
-      ks.issue(keys.key0(i + 1), k_st1, wave);
-      vs.issue(keys.key0(i + 1), v_st1, wave);
-    }
-    stage(k_st0, v_st0, i);
+  for (int i = 0; i < n_all; i += 4) {
+    ready(i);
+    issue(i + 3, k3_, v3_);
+    step(k0_, v0_, k1_, i);
     if (i + 1 >= n_all) break;
-    stage_ready();
-    if (i + 2 < n_all) {
-      ks.issue(keys.key0(i + 2), k_st0, wave);
-      vs.issue(keys.key0(i + 2), v_st0, wave);
-    }
-    stage(k_st1, v_st1, i + 1);
+    ready(i + 1);
+    issue(i + 4, k0_, v0_);
+    step(k1_, v1_, k2_, i + 1);
+    if (i + 2 >= n_all) break;
+    ready(i + 2);
+    issue(i + 5, k1_, v1_);
+    step(k2_, v2_, k3_, i + 2);
+    if (i + 3 >= n_all) break;
+    ready(i + 3);
+    issue(i + 6, k2_, v2_);
+    step(k3_, v3_, k0_, i + 3);
   }
 
   const bool met = row_in && !sum_finite(acc);
@@ -352,13 +454,14 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
     SinkArgs A) {
   using C = SinkBwdCfg<D, E>;
   using T = SinkTile<D, E, (D >= 128)>;
-  using Stage = SinkStage<D, E, C::STAGE, 256>;
+  using Stage = SinkStage<D, E, C::ROWS, 256>;
   using LdsT = typename T::LdsT;
   constexpr int ND = T::ND;
-  __shared__ __attribute__((aligned(1024))) LdsT q_st0[C::STAGE * D];
-  __shared__ __attribute__((aligned(1024))) LdsT g_st0[C::STAGE * D];
-  __shared__ __attribute__((aligned(1024))) LdsT q_st1[C::STAGE * D];
-  __shared__ __attribute__((aligned(1024))) LdsT g_st1[C::STAGE * D];
+  __shared__ __attribute__((aligned(1024))) LdsT q_st0[C::ROWS * D];
+  __shared__ __attribute__((aligned(1024))) LdsT g_st0[C::ROWS * D];
+  __shared__ __attribute__((aligned(1024))) LdsT q_st1[C::ROWS * D];
+  __shared__ __attribute__((aligned(1024))) LdsT g_st1[C::ROWS * D];
+  __shared__ __attribute__((aligned(16))) typename T::Frag v_rows[C::V_LDS ? 256 : 1];
   __shared__ __attribute__((aligned(256))) float stat0[2 * 64];  // lse2, then delta
   __shared__ __attribute__((aligned(256))) float stat1[2 * 64];
 
@@ -393,7 +496,7 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
   const int p_last = min(si.base + A.q_len, A.kv_len) - 1;
   const int p_lo = max(j0, si.base);
   const int p_hi = j0 < sink_end ? p_last : min(p_last, j0 + 127 + W - 1);
-  const int per_head = p_hi >= p_lo ? (p_hi - p_lo) / C::STAGE + 1 : 0;
+  const int per_head = p_hi >= p_lo ? (p_hi - p_lo) / C::ROWS + 1 : 0;
   const int64_t total = (int64_t)per_head * A.groups;
   const int s0 = (int)(total * it.chunk / it.n_chunks);
   const int s1 = (int)(total * (it.chunk + 1) / it.n_chunks);
@@ -409,6 +512,12 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
               key_in, A.d_real);
   t.load_frag(vf, at<E>(A.v, (int64_t)b * A.vsb + (int64_t)kvh * A.vsh + (int64_t)j * A.vss),
               key_in, A.d_real);
+  // (a lane reads back what it wrote)
+  u32x4* const v_own = (u32x4*)v_rows + (wave * (int)(sizeof(vf) / 16) * 64 + lane);
+  if constexpr (C::V_LDS) {
+#pragma unroll
+    for (int s = 0; s < T::NS; ++s) v_own[64 * s] = __builtin_bit_cast(u32x4, vf.f[s]);
+  }
   f32x16 dk[ND], dv[ND];
 #pragma unroll
   for (int d = 0; d < ND; ++d) dk[d] = dv[d] = f32x16{};
@@ -419,10 +528,15 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
   gs.init(nullptr, A.doss, A.q_len, A.d_real, tid);
   int head = per_head > 0 ? s0 / per_head : 0, at_stage = s0 - head * per_head;
   int staged = -1;
+  // Stage `at` of a head is, of the block's, the one whose number among all rows
+  // is at modulo per_head: blocks that run side by side read the same rows at the
+  // same time (8192 rows of 4 heads, window 1024: 875 MB from beyond L2, 350 so)
+  const int turn = per_head > 0 ? (p_lo - si.base) / C::ROWS % per_head : 0;
   // the next stage in order -> buffers; returns its first row
   auto issue = [&](LdsT* qd, LdsT* gd, float* stat) __attribute__((always_inline)) {
     const int h = kvh * A.groups + head;
-    const int row0 = p_lo - si.base + at_stage * C::STAGE;
+    const int k = at_stage - turn + (at_stage < turn ? per_head : 0);
+    const int row0 = p_lo - si.base + k * C::ROWS;
     if (h != staged) {  // another head's rows
       qs.rebase(at<E>(A.q, (int64_t)b * A.qsb + (int64_t)h * A.qsh));
       gs.rebase(at<E>(A.dout, (int64_t)b * A.dosb + (int64_t)h * A.dosh));
@@ -450,32 +564,128 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
                    __attribute__((always_inline)) {
     const int p0 = si.base + row0 + 32 * rb, p1 = min(p0 + 31, p_last);
     if (p0 > p_last || none_seen(p0, p1, jw0, W, sink_end)) return;
+    const bool whole = p0 + 31 <= p_last && all_seen(p0, p0 + 31, jw0, W, sink_end);
+    auto hide = [&](f32x16& s) __attribute__((always_inline)) {
+      uint32_t m[16];
+      key_masks<0>(m, seen_rows(j, p0, p_last, W, sink_end) >> (4 * hf));
+      mask_select(s, m);
+    };
+    auto row_stat = [&](int at, int q4) __attribute__((always_inline)) {
+      return *(const f32x4*)(stat + at + 32 * rb + 8 * q4 + 4 * hf);
+    };
     f32x16 s = f32x16{}, dp = f32x16{};
-    if (p0 + 31 > p_last || !all_seen(p0, p0 + 31, jw0, W, sink_end))
-      mask_init<0>(s, ~(seen_rows(j, p0, p_last, W, sink_end) >> (4 * hf)));
-    // (one product's operands at a time: the accumulators, K and V leave room
-    // for no more)
-    t.row_product(s, qb, rb, kf);
-    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (T::ES == 2) {
+      // The four products in written order, each beside the vector work of the
+      // one before it (S: none; dP: P's exponentials; dV: dS; dK: dS's rest),
+      // operands read AHEAD products ahead.
+      constexpr int AHEAD = 3, NS = T::NS, PER = 8 / NS;  // products of each; pairs of rows a product
+      typename T::V8 qa[NS], ga[NS], va[NS];
+      int base;  // of the reads' addresses
+      u32x4 gc[NS], qc[NS];
+      typename T::P pp, pd;
+      f32x4 l2[4], dl[4];
+      auto read = [&](int i) __attribute__((always_inline)) {  // operands in their order
+        const int k = i % NS;
+        if (i < 2 * NS) {
+          if (k == 0) base = T::fresh(t.ra[0]);
+          if (i < NS) {
+            qa[k] = t.row_operand(qb, rb, k, base);
+          } else {
+            ga[k] = t.row_operand(gb, rb, k, base);
+            if constexpr (C::V_LDS) va[k] = __builtin_bit_cast(typename T::V8, v_own[64 * k]);
+          }
+        } else if (i < 4 * NS) {
+          if (k % ND == 0) base = T::fresh(t.ca[0]);
+          if (i < 3 * NS)
+            gc[k] = t.col_operand(gb, rb, k % ND, k / ND, base);
+          else
+            qc[k] = t.col_operand(qb, rb, k % ND, k / ND, base);
+        }
+      };
+      auto exps = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f32x4 l2 = *(const f32x4*)(stat + 32 * rb + 8 * q + 4 * hf);
+        for (int q = k * PER; q < (k + 1) * PER; ++q) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        s[4 * q + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + e], scale, -l2[e]));
+          for (int e = 2 * q; e < 2 * q + 2; ++e)
+            s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], scale, -l2[e / 4][e % 4]));
+          pp.w[q] = T::M::pack2(s[2 * q], s[2 * q + 1]);
+        }
+      };
+      auto grads = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = k * PER; q < (k + 1) * PER; ++q) {
+#pragma unroll
+          for (int e = 2 * q; e < 2 * q + 2; ++e) s[e] *= dp[e] - dl[e / 4][e % 4];
+          pd.w[q] = T::M::pack2(s[2 * q], s[2 * q + 1]);
+        }
+      };
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) read(k);
+#pragma unroll
+      for (int k = 0; k < NS; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        s = T::M::mfma32(qa[k], kf.f[k], s);
+        read(k + AHEAD);
+      }
+      l2[0] = row_stat(0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      if (!whole) hide(s);
+#pragma unroll
+      for (int k = 0; k < NS; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        dp = T::M::mfma32(ga[k], C::V_LDS ? va[k] : vf.f[k], dp);
+        read(NS + k + AHEAD);
+        if (PER == 2 || k % 2 == 0) {
+          const int q4 = (k * PER) / 2 + 1;
+          if (q4 < 4) l2[q4] = row_stat(0, q4);
+        }
+        if (k > 0) exps(k - 1);
+      }
+      dl[0] = row_stat(64, 0);
+#pragma unroll
+      for (int k = 0; k < NS; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        T::col_step(dv[k % ND], gc[k], pp, k / ND);
+        read(2 * NS + k + AHEAD);
+        if (PER == 2 || k % 2 == 0) {
+          const int q4 = (k * PER) / 2 + 1;
+          if (q4 < 4) dl[q4] = row_stat(64, q4);
+        }
+        if (k == 0) exps(NS - 1);
+        if (k > 0) grads(k - 1);
+      }
+#pragma unroll
+      for (int k = 0; k < NS; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (k == 0) grads(NS - 1);
+        T::col_step(dk[k % ND], qc[k], pd, k / ND);
+        read(3 * NS + k + AHEAD);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    } else {
+      t.row_product(s, qb, rb, kf);
+      __builtin_amdgcn_sched_barrier(0);
+      if (!whole) hide(s);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 l2 = row_stat(0, q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          s[4 * q + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + e], scale, -l2[e]));
+      }
+      t.row_product(dp, gb, rb, vf);
+      __builtin_amdgcn_sched_barrier(0);
+      t.col_product(dv, gb, rb, t.pack(s));
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 dl = row_stat(64, q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[4 * q + e] = s[4 * q + e] * (dp[4 * q + e] - dl[e]);
+      }
+      t.col_product(dk, qb, rb, t.pack(dp));
+      __builtin_amdgcn_sched_barrier(0);
     }
-    t.row_product(dp, gb, rb, vf);
-    __builtin_amdgcn_sched_barrier(0);
-    t.col_product(dv, gb, rb, t.pack(s));
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f32x4 dl = *(const f32x4*)(stat + 64 + 32 * rb + 8 * q + 4 * hf);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) dp[4 * q + e] = s[4 * q + e] * (dp[4 * q + e] - dl[e]);
-    }
-    t.col_product(dk, qb, rb, t.pack(dp));
-    __builtin_amdgcn_sched_barrier(0);
   };
   int row_a = 0, row_b = 0;
   if (s0 < s1) row_a = issue(q_st0, g_st0, stat0);
@@ -483,12 +693,12 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
     stage_ready();
     if (i + 1 < s1) row_b = issue(q_st1, g_st1, stat1);
 #pragma unroll
-    for (int rb = 0; rb < C::NB; ++rb) block(q_st0, g_st0, stat0, rb, row_a);
+    for (int rb = 0; rb < C::ROWS / 32; ++rb) block(q_st0, g_st0, stat0, rb, row_a);
     if (i + 1 >= s1) break;
     stage_ready();
     if (i + 2 < s1) row_a = issue(q_st0, g_st0, stat0);
 #pragma unroll
-    for (int rb = 0; rb < C::NB; ++rb) block(q_st1, g_st1, stat1, rb, row_b);
+    for (int rb = 0; rb < C::ROWS / 32; ++rb) block(q_st1, g_st1, stat1, rb, row_b);
   }
 
   if (it.n_chunks > 1) {  // a part: [wave][dK, dV][d block][register][lane]
