@@ -178,6 +178,13 @@ void sink_pattern(SinkArgs& g, const esa_window* w) {
   g.nqb = (g.q_len + 127) / 128;
 }
 
+// Workgroups of the forward that the chip runs at a time, and of dK / dV's kernel
+// (as many a CU as its registers hold)
+int64_t sink_fwd_slots(const SinkArgs& g) {
+  return 256 * (g.elem == ESA_F32 ? (g.d_real > 64 ? 1 : 2) : g.d_real > 64 ? 2 : 4);
+}
+int64_t sink_kv_slots(const SinkArgs& g) { return g.elem == ESA_F32 && g.d_real > 64 ? 256 : 512; }
+
 // Keys that a call's rows walk, at most.
 int64_t sink_keys(const SinkArgs& g) {
   return std::min<int64_t>(g.kv_len, (int64_t)g.window + g.sinks + g.q_len);
@@ -200,7 +207,7 @@ bool sink_decodes(const SinkArgs& g) {
   const bool f32 = g.elem == ESA_F32;
   const double keys = (double)sink_keys(g);
   const double tiles = (double)g.B * g.Hkv * (((int64_t)g.groups * g.q_len + 15) / 16);
-  const int64_t blocks = (int64_t)g.B * g.H * g.nqb, slots = f32 ? 256 : 512;
+  const int64_t blocks = (int64_t)g.B * g.H * g.nqb, slots = sink_fwd_slots(g);
   const double rate = (f32 ? 2500.0 : 13500.0) * (g.d_real <= 64 ? 2.0 : 1.0);
   return tiles * keys / rate + 8.0 < keys * (f32 ? 0.08 : 0.022) * (double)((blocks + slots - 1) / slots)
          || (int64_t)g.groups * g.q_len <= 16;
@@ -267,7 +274,7 @@ int sink_qpad(int q_len) { return (q_len + 3) / 4 * 4; }
 void sink_bwd_plan(SinkArgs& g) {
   g.nkb = (g.kv_len + 127) / 128;
   g.qpad = sink_qpad(g.q_len);
-  const int64_t slots = g.elem == ESA_F32 ? 256 : 512, part = 6;
+  const int64_t slots = sink_kv_slots(g), part = g.elem == ESA_F32 ? 1 : 6;
   const int64_t kv = (int64_t)g.B * g.Hkv;
   const int n_sink = std::min(g.nkb, (g.sinks + 127) / 128);
   auto stages = [&](int64_t rows) { return (rows + 63) / 64 * g.groups; };

@@ -302,6 +302,24 @@ struct SinkTile {
     v[3] = (typename M::s)e;
     *(typename M::v4*)((uint16_t*)row + dim) = v;
   }
+  // scale * x, one 32-dim block of an accumulator, to dims dim0 .. of the lane's
+  // row: the row's two lanes trade halves and store 16 bytes each (with 8 a lane
+  // the stores of 128 rows took as long as three stages)
+  static __device__ __forceinline__ void store32(void* row, int dim0, const f32x16& x, float scale,
+                                                 int hf, int d_real, bool in) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      uint32_t w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        w[q] = M::pack2(x[8 * j + 2 * q] * scale, x[8 * j + 2 * q + 1] * scale);
+      const auto a = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+      const auto b = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+      const int dim = dim0 + 16 * j + 8 * hf;
+      if (in && dim < d_real)
+        *(u32x4*)((uint16_t*)row + dim) = u32x4{a[0], b[0], a[1], b[1]};
+    }
+  }
   static __device__ __forceinline__ float rounded(float x) { return (float)(typename M::s)x; }
   static __device__ __forceinline__ float psum(const P& p, float c) {
 #pragma unroll
@@ -381,6 +399,16 @@ struct SinkTile<D, Elem::f32, TIGHT> {
   static __device__ __forceinline__ void store4(void* row, int dim, float a, float b, float c,
                                                 float e) {
     *(f32x4*)((float*)row + dim) = f32x4{a, b, c, e};
+  }
+  static __device__ __forceinline__ void store32(void* row, int dim0, const f32x16& x, float scale,
+                                                 int hf, int d_real, bool in) {
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      const int dim = dim0 + 8 * q4 + 4 * hf;
+      if (in && dim < d_real)
+        store4(row, dim, x[4 * q4] * scale, x[4 * q4 + 1] * scale, x[4 * q4 + 2] * scale,
+               x[4 * q4 + 3] * scale);
+    }
   }
   static __device__ __forceinline__ float rounded(float x) { return x; }
   static __device__ __forceinline__ float psum(const P& p, float c) {
@@ -512,6 +540,19 @@ __device__ __forceinline__ void store_out4(const SinkArgs& A, int64_t row, int d
   if (A.ores)
     T::store4((char*)A.ores + row * T::ES, dim, a - T::rounded(a), b - T::rounded(b),
               c - T::rounded(c), d - T::rounded(d));
+}
+
+// The same of a 32-dim block of accumulators.
+template <int D, Elem E>
+__device__ __forceinline__ void store_out32(const SinkArgs& A, int64_t row, int dim0, f32x16 x,
+                                            float scale, int hf, bool in) {
+  using T = SinkTile<D, E>;
+  T::store32((char*)A.o + row * T::ES, dim0, x, scale, hf, A.d_real, in);
+  if (A.ores) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = x[e] * scale - T::rounded(x[e] * scale);
+    T::store32((char*)A.ores + row * T::ES, dim0, x, 1.f, hf, A.d_real, in);
+  }
 }
 
 // Row `row` of one head from its own keys, by one wave: lanes take 64 keys at a

@@ -36,12 +36,15 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D, Elem E>
 struct SinkBwdCfg {
-  // dK / dV: where K, V, their gradients and the products would take more than
-  // the 256 registers of a wave in a pair (head_dim 128, 16-bit), V's rows are
-  // kept in LDS, and stages are 32 rows, so that two workgroups' still fit
-  static constexpr bool V_LDS = E != Elem::f32 && D >= 128;
-  static constexpr int ROWS = E == Elem::f32 || V_LDS ? 32 : 64;
-  static constexpr int WAVES_PER_SIMD = E == Elem::f32 ? 1 : 2;
+  // waves a SIMD: what the registers allow (dK / dV at head_dim 64 in 16 bits
+  // gains nothing from a third: 195 us against 191)
+  static constexpr int DQ_WAVES = E == Elem::f32 ? (D >= 128 ? 1 : 2) : D >= 128 ? 2 : 3;
+  static constexpr int KV_WAVES = E == Elem::f32 && D >= 128 ? 1 : 2;
+  // dK / dV: where K, V, their gradients and the products take more registers
+  // than half a SIMD's, V's rows are kept in LDS, and stages are 32 rows, so that
+  // two workgroups' still fit
+  static constexpr bool V_LDS = KV_WAVES == 2 && (E == Elem::f32 || D >= 128);
+  static constexpr int ROWS = E == Elem::f32 || D >= 128 ? 32 : 64;
 };
 
 template <Elem E>
@@ -89,7 +92,7 @@ __device__ void fix_dq_row(const SinkArgs& A, int b, int h, int kvh, int row, in
 }
 
 template <int D, Elem E>
-__global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_dq_kernel(
+__global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::DQ_WAVES)) void sink_dq_kernel(
     SinkArgs A) {
   using T = SinkTile<D, E>;
   using Stage = SinkStage<D, E, 32, 256>;
@@ -287,19 +290,11 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
   }
 
   const bool met = row_in && !sum_finite(acc);
-  if (row_in) {
-    auto* row = (typename ElemT<E>::T*)A.dq + (int64_t)b * A.dqsb + (int64_t)h * A.dqsh +
-                (int64_t)r * A.dqss;
+  auto* dq = (typename ElemT<E>::T*)A.dq + (int64_t)b * A.dqsb + (int64_t)h * A.dqsh +
+             (int64_t)r * A.dqss;
 #pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const int dim = 32 * d + 8 * q4 + 4 * hf;
-        if (dim < A.d_real)
-          T::store4(row, dim, acc[d][4 * q4] * A.sm_scale, acc[d][4 * q4 + 1] * A.sm_scale,
-                    acc[d][4 * q4 + 2] * A.sm_scale, acc[d][4 * q4 + 3] * A.sm_scale);
-      }
-  }
+  for (int d = 0; d < ND; ++d)
+    T::store32(dq, 32 * d, acc[d], A.sm_scale, hf, A.d_real, row_in);
   uint64_t bad = __builtin_amdgcn_ballot_w64(met);
   bad = (bad | bad >> 32) & 0xffffffffull;
   if (bad) __builtin_amdgcn_s_waitcnt(0);  // the stores above come first
@@ -360,29 +355,21 @@ __device__ __forceinline__ KeyItem key_item(const SinkArgs& A) {
   return key_block(A, kv0 + kv, cls, block, u - block * A.cls_cut[cls]);
 }
 
-// Stores 32 keys' dK^T and dV^T (one wave's accumulators)
+// Stores 32 keys' dK^T and dV^T (one wave's accumulators; in: the lane's key is one)
 template <int D, Elem E>
 __device__ __forceinline__ void store_keys(const SinkArgs& A, int b, int kvh, int j, int hf,
                                            const f32x16 (&dk)[SinkTile<D, E>::ND],
-                                           const f32x16 (&dv)[SinkTile<D, E>::ND]) {
+                                           const f32x16 (&dv)[SinkTile<D, E>::ND], bool in) {
   using T = SinkTile<D, E>;
   auto* kr = (typename ElemT<E>::T*)A.dk + (int64_t)b * A.dksb + (int64_t)kvh * A.dksh +
              (int64_t)j * A.dkss;
   auto* vr = (typename ElemT<E>::T*)A.dv + (int64_t)b * A.dvsb + (int64_t)kvh * A.dvsh +
              (int64_t)j * A.dvss;
-  const float c = A.sm_scale;
 #pragma unroll
-  for (int d = 0; d < T::ND; ++d)
-#pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4) {
-      const int dim = 32 * d + 8 * q4 + 4 * hf;
-      if (dim < A.d_real) {
-        T::store4(kr, dim, dk[d][4 * q4] * c, dk[d][4 * q4 + 1] * c, dk[d][4 * q4 + 2] * c,
-                  dk[d][4 * q4 + 3] * c);
-        T::store4(vr, dim, dv[d][4 * q4], dv[d][4 * q4 + 1], dv[d][4 * q4 + 2],
-                  dv[d][4 * q4 + 3]);
-      }
-    }
+  for (int d = 0; d < T::ND; ++d) {
+    T::store32(kr, 32 * d, dk[d], A.sm_scale, hf, A.d_real, in);
+    T::store32(vr, 32 * d, dv[d], 1.f, hf, A.d_real, in);
+  }
 }
 
 // dK and dV of one key from the rows that see it, by one wave
@@ -450,7 +437,7 @@ __device__ __forceinline__ void fix_keys(const SinkArgs& A, const SeqInfo& si, i
 }
 
 template <int D, Elem E>
-__global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_dkdv_kernel(
+__global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::KV_WAVES)) void sink_dkdv_kernel(
     SinkArgs A) {
   using C = SinkBwdCfg<D, E>;
   using T = SinkTile<D, E, (D >= 128)>;
@@ -513,10 +500,11 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
   t.load_frag(vf, at<E>(A.v, (int64_t)b * A.vsb + (int64_t)kvh * A.vsh + (int64_t)j * A.vss),
               key_in, A.d_real);
   // (a lane reads back what it wrote)
-  u32x4* const v_own = (u32x4*)v_rows + (wave * (int)(sizeof(vf) / 16) * 64 + lane);
+  constexpr int PIECES = sizeof(vf) / 16;
+  u32x4* const v_own = (u32x4*)v_rows + (wave * PIECES * 64 + lane);
   if constexpr (C::V_LDS) {
 #pragma unroll
-    for (int s = 0; s < T::NS; ++s) v_own[64 * s] = __builtin_bit_cast(u32x4, vf.f[s]);
+    for (int s = 0; s < PIECES; ++s) v_own[64 * s] = __builtin_bit_cast(u32x4, vf.f[s]);
   }
   f32x16 dk[ND], dv[ND];
 #pragma unroll
@@ -673,6 +661,10 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
         for (int e = 0; e < 4; ++e)
           s[4 * q + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + e], scale, -l2[e]));
       }
+      if constexpr (C::V_LDS) {
+#pragma unroll
+        for (int s = 0; s < PIECES; ++s) vf.f[s] = __builtin_bit_cast(f32x4, v_own[64 * s]);
+      }
       t.row_product(dp, gb, rb, vf);
       __builtin_amdgcn_sched_barrier(0);
       t.col_product(dv, gb, rb, t.pack(s));
@@ -713,7 +705,7 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
     return;
   }
   const bool met = key_in && !(sum_finite(dk) && sum_finite(dv));
-  if (key_in) store_keys<D, E>(A, b, kvh, j, hf, dk, dv);
+  store_keys<D, E>(A, b, kvh, j, hf, dk, dv, key_in);
   fix_keys<E>(A, si, b, kvh, jw0, sink_end, met, lane);
 }
 
@@ -763,13 +755,7 @@ __global__ __launch_bounds__(256) void sink_join_kernel(SinkArgs A) {
                            (int64_t)it.kvh * A.dksh + (int64_t)j * A.dkss
                      : (typename ElemT<E>::T*)A.dv + (int64_t)it.b * A.dvsb +
                            (int64_t)it.kvh * A.dvsh + (int64_t)j * A.dvss;
-#pragma unroll
-    for (int q4 = 0; q4 < 4; ++q4) {
-      const int dim = 32 * d + 8 * q4 + 4 * hf;
-      if (key_in && dim < A.d_real)
-        T::store4(row, dim, x[4 * q4] * scale, x[4 * q4 + 1] * scale, x[4 * q4 + 2] * scale,
-                  x[4 * q4 + 3] * scale);
-    }
+    T::store32(row, 32 * d, x, scale, hf, A.d_real, key_in);
   }
   // a key that met a non-finite value, again from its own rows (by one wave,
   // after every wave's stores)

@@ -18,7 +18,8 @@ namespace {
 
 template <int D, Elem E>
 struct SinkFwdCfg {
-  static constexpr int WAVES_PER_SIMD = E == Elem::f32 ? 1 : 2;
+  static constexpr int WAVES_PER_SIMD =
+      E == Elem::f32 ? (D >= 128 ? 1 : 2) : D >= 128 ? 2 : 4;
 };
 
 template <int D, Elem E>
@@ -138,8 +139,8 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
       auto exps = [&](int q) __attribute__((always_inline)) {  // two of the 16
         s[2 * q] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * q], scale, -m_use));
         s[2 * q + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * q + 1], scale, -m_use));
-        l_run += s[2 * q];
-        l_run += s[2 * q + 1];
+        l_run += s[2 * q] + s[2 * q + 1];
+        asm volatile("" : "+v"(l_run));  // summed here, not behind the last product
         pp.w[q] = T::M::pack2(s[2 * q], s[2 * q + 1]);
       };
       constexpr int H = T::NS / 2, EH = 4 / H > 0 ? 4 / H : 1;  // exponential pairs a product
@@ -173,6 +174,7 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
           n_run = T::M::dot2(pp.w[2 * k + 4], n_run);
           n_run = T::M::dot2(pp.w[2 * k + 5], n_run);
         }
+        asm volatile("" : "+v"(n_run));
       }
       top = row_top(sn);
       __builtin_amdgcn_sched_barrier(0);
@@ -242,28 +244,19 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
   const bool met = row_in && !(sum_finite(oacc) && __builtin_isfinite(l_run));
   const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
   const float n_tot = n_run + __shfl_xor(n_run, 32, 64);
-  if (row_in) {
-    // a row that sees no key (before the sequence's first one): 0 and -inf;
-    // one without a place in the cache: NaN
-    const bool valid = row_valid(A, si, b, r);
-    float inv = 1.f / n_tot, lse = (m_run + __log2f(l_tot)) * 0.69314718055994530942f;
-    if (p < f) {
-      inv = 0.f;
-      lse = -INFINITY;
-    }
-    if (!valid) inv = lse = __builtin_nanf("");
-    const int64_t orow = (int64_t)b * A.osb + (int64_t)h * A.osh + (int64_t)r * A.oss;
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-#pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4) {
-        const int dim = 32 * d + 8 * q4 + 4 * hf;
-        if (dim < A.d_real)
-          store_out4<D, E>(A, orow, dim, oacc[d][4 * q4] * inv, oacc[d][4 * q4 + 1] * inv,
-                           oacc[d][4 * q4 + 2] * inv, oacc[d][4 * q4 + 3] * inv);
-      }
-    if (A.lse && hf == 0) A.lse[(int64_t)b * A.lsb + (int64_t)h * A.lsh + r] = lse;
+  // a row that sees no key (before the sequence's first one): 0 and -inf; one
+  // without a place in the cache: NaN
+  const bool valid = row_in && row_valid(A, si, b, r);
+  float inv = 1.f / n_tot, lse = (m_run + __log2f(l_tot)) * 0.69314718055994530942f;
+  if (p < f) {
+    inv = 0.f;
+    lse = -INFINITY;
   }
+  if (!valid) inv = lse = __builtin_nanf("");
+  const int64_t orow = (int64_t)b * A.osb + (int64_t)h * A.osh + (int64_t)r * A.oss;
+#pragma unroll
+  for (int d = 0; d < ND; ++d) store_out32<D, E>(A, orow, 32 * d, oacc[d], inv, hf, row_in);
+  if (row_in && A.lse && hf == 0) A.lse[(int64_t)b * A.lsb + (int64_t)h * A.lsh + r] = lse;
   // ---- rows that met a non-finite value, again from their own keys
   uint64_t bad = __builtin_amdgcn_ballot_w64(met);
   bad = (bad | bad >> 32) & 0xffffffffull;
