@@ -29,6 +29,7 @@ from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from elastic_sparse_attention import _dtype_code, _prep, _require_gpu, _stream
 from esa_native import EsaRotaryArgs, check, load
@@ -78,7 +79,11 @@ def _check_qk(q: torch.Tensor, k: torch.Tensor) -> None:
 
 
 def _positions_2d(positions, batch: int, rows: int, device: torch.device) -> torch.Tensor:
-    """positions as int64 on ``device``: [rows] (shared) or [batch, rows]."""
+    """positions as int64 on ``device``: [rows] (shared) or [batch, rows]; None
+    is row r at position r (formed for the call: nothing is kept that another
+    stream, or a graph's memory, would have to have finished first)."""
+    if positions is None:
+        return torch.arange(rows, device=device)
     if not isinstance(positions, torch.Tensor):
         positions = torch.as_tensor(positions)
     pos = positions
@@ -156,7 +161,7 @@ def qk_norm_rope_fwd(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.
     """q and k normed and rotated: new tensors of their shapes and dtype.
 
     ``positions``: int64 ``[n]`` (shared by the batch) or ``[B, n]``, any
-    values; ``inv_freq``: float64 ``[rotary_dim / 2]`` on the rows' device,
+    values, or None (row r is position r); ``inv_freq``: float64 ``[rotary_dim / 2]`` on the rows' device,
     radians per position; a weight of None is 1."""
     _check_qk(q, k)
     B, _, n, D = q.shape
@@ -262,6 +267,8 @@ def check_cache_position(cache_position, batch: int, rows: int, kv_len: int,
     """cache_position as int64 on ``device``, ``[rows]`` or ``[batch, rows]``.
     A host-side value is checked: IndexError outside the cache, ValueError
     where a sequence's rows do not follow each other."""
+    if cache_position is None:
+        raise ValueError("cache_position must say where the rows are")
     on_gpu = isinstance(cache_position, torch.Tensor) and cache_position.is_cuda
     if not on_gpu:
         pos = _positions_2d(cache_position, batch, rows, torch.device("cpu"))
@@ -285,6 +292,7 @@ class _QKNormRopeFunction(torch.autograd.Function):
         return qk_norm_rope_fwd(q, k, q_weight, k_weight, inv_freq, positions, eps, interleaved)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gq, gk):
         q, k, qw, kw, inv_freq, positions = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -331,7 +339,6 @@ class QKNormRope(nn.Module):
         half = rotary_dim // 2
         inv_freq = base ** (-torch.arange(half, dtype=torch.float64) / half)
         self.register_buffer("inv_freq", inv_freq, persistent=False)
-        self._arange: Optional[torch.Tensor] = None  # positions of whole sequences
 
     def _apply(self, fn, *args, **kwargs):
         # the frequencies stay float64 under .half(), .bfloat16() and .to(dtype):
@@ -343,10 +350,10 @@ class QKNormRope(nn.Module):
             self._buffers["inv_freq"] = freq.to(moved.device)
         return self
 
-    def forward(self, q: torch.Tensor, k: torch.Tensor, positions) -> Tuple[torch.Tensor,
-                                                                            torch.Tensor]:
+    def forward(self, q: torch.Tensor, k: torch.Tensor, positions=None
+                ) -> Tuple[torch.Tensor, torch.Tensor]:
         """q ``[B, H, n, D]`` and k ``[B, Hkv, n, D]`` normed and rotated at
-        ``positions`` (``[n]`` or ``[B, n]``)."""
+        ``positions`` (``[n]`` or ``[B, n]``; None: row r is position r)."""
         self._check_dim(q)
         positions = _positions_2d(positions, q.shape[0], q.shape[2], q.device)
         if torch.is_grad_enabled() and any(
@@ -376,11 +383,7 @@ class QKNormRope(nn.Module):
             if cache_position is not None:
                 raise ValueError("a layer with `rotary` takes cache_position together with "
                                  "kv_cache: its k and v are the new rows")
-            n = q.shape[2]
-            if self._arange is None or self._arange.numel() != n or \
-                    self._arange.device != q.device:
-                self._arange = torch.arange(n, device=q.device)
-            q, k = self(q, k, self._arange)
+            q, k = self(q, k)
             return q, k, v
         if cache_position is None:
             raise ValueError("kv_cache needs cache_position")

@@ -372,3 +372,36 @@ def test_replayed_graph_and_another_stream():
         y = layer(q, k, pos)[0]
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(y, ref)
+
+
+def test_rows_in_order_without_positions():
+    """No positions: row r at r, also where a layer's first call is captured
+    and another length, then the captured one again, follow eagerly."""
+    layer = QKNormRope(64).to(DEV).to(BF16)
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    q = torch.randn(2, 4, 21, 64, generator=gen, device=DEV).to(BF16)
+    k = torch.randn(2, 2, 21, 64, generator=gen, device=DEV).to(BF16)
+    with torch.no_grad():
+        want = layer(q, k, torch.arange(21))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = layer.attention_rows(q, k, k, None, None)
+        for _ in range(3):
+            got = layer.attention_rows(q, k, k, None, None)
+            short = layer(q[:, :, :5], k[:, :, :5])
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+            assert torch.equal(short[0], want[0][:, :, :5])
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_no_second_derivative():
+    layer = QKNormRope(64).to(DEV)
+    q = torch.randn(1, 2, 3, 64, device=DEV, requires_grad=True)
+    y, _ = layer(q, q, torch.arange(3))
+    (g,) = torch.autograd.grad(y.square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.square().sum().backward()
