@@ -26,6 +26,7 @@ from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from elastic_sparse_attention import (_check_qkv, _dtype_code, _fwd_args, _prep, _require_gpu)
 from esa_native import EsaBwdArgs, EsaWindow, check, load
@@ -163,6 +164,8 @@ def sink_window_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         raise ValueError(f"o and dout must be [{B}, {Lq}, {H}, {D}] and lse [{B}, {H}, {Lq}]; got "
                          f"{list(o.shape)}, {list(dout.shape)} and {list(lse.shape)}")
     _require_gpu(o, lse, dout)
+    if not (o.device == lse.device == dout.device == q.device):
+        raise ValueError("o, lse and dout must be on q's device")
     if o.dtype != q.dtype or lse.dtype != torch.float32:
         raise ValueError("o must have q's dtype and lse float32, as the forward returns them")
     if o_residual is not None:
@@ -220,6 +223,7 @@ class _SinkWindowFunction(torch.autograd.Function):
         return o
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do):
         q, k, v, o, lse, res, positions, first_key = ctx.saved_tensors
         dq, dk, dv = _bwd(q, k, v, o, lse, do, ctx.window, ctx.num_sinks, ctx.scaling, positions,

@@ -513,3 +513,80 @@ def test_replayed_graph_and_another_stream():
         have = train()
     torch.cuda.current_stream().wait_stream(side)
     assert all(torch.equal(a, b) for a, b in zip(have, want))
+
+
+def random_case(seed):
+    """One call over everything that a call may vary."""
+    import random
+    r = random.Random(seed)
+    B, Hkv, G = r.choice([1, 2, 3]), r.choice([1, 2]), r.choice([1, 2, 3, 5])
+    dtype = r.choice([BF16, BF16, F16, F32])
+    D = r.choice([8, 24, 64, 72, 104, 128]) if dtype != F32 else r.choice([4, 20, 64, 100, 128])
+    Lk = r.choice([1, 31, 127, 129, 400, 641, 1100])
+    Lq = Lk if r.random() < 0.5 else r.choice([1, 2, 9, 33, 128, Lk])
+    Lq = min(Lq, Lk)
+    start = [0] * B if Lq == Lk else [r.randint(0, Lk - Lq) for _ in range(B)]
+    first = None if r.random() < 0.5 else [r.choice([0, r.randint(0, Lk), Lk]) for _ in range(B)]
+    W = r.choice([1, 5, 32, 33, 100, 128, 500, 1 << 20])
+    S = r.choice([0, 1, 4, 31, 128, 200])
+    return B, Hkv * G, Hkv, Lq, Lk, D, W, S, dtype, start, first, r.random() < 0.5
+
+
+def gradual(q, k, v, g, seen, scale, dtype):
+    """What the bounds take on where values fall below the type's normal range
+    (float16: 2^-14).  Spacing there is smallest_normal * eps whatever the value,
+    so a rounding is off by up to half of that, `least` (2^-25), not u |x|: each
+    output by least, and a product of probabilities or dS by least times the sum
+    of what they meet (the forward's probabilities are divided by a sum >= 1)."""
+    t = torch.finfo(dtype)
+    least = t.smallest_normal * t.eps / 2
+    G = q.shape[1] // k.shape[1]
+    B, H, Lq, D = q.shape
+    kk, vv = (x.double().abs().repeat_interleave(G, 1) for x in (k, v))
+    vis = seen[:, None].double()
+    fold = lambda x: x.view(B, H // G, G, *x.shape[2:]).sum(2)
+    o, dq = least * (1 + vis @ vv), least * (1 + scale * (vis @ kk))
+    dk = least * (1 + fold(scale * (vis.transpose(2, 3) @ q.double().abs())))
+    dv = least * (1 + fold(vis.transpose(2, 3) @ g.double().abs()))
+    return o, 0.0, dq, dk, dv
+
+
+def run_case(B, H, Hkv, Lq, Lk, D, W, S, dtype, start, first, strided, seed):
+    q, k, v, gen = make(B, H, Hkv, Lq, Lk, D, dtype, strided, seed)
+    g = rows(B, H, Lq, D, dtype, gen, True)
+    f = torch.zeros(B, dtype=torch.int64) if first is None else torch.tensor(first)
+    pos = torch.tensor(start)[:, None] + torch.arange(Lq)
+    seen = window_mask(pos, f, Lk, W, S)
+    ref, tol = bounds(q, k, v, seen, D ** -0.5, dtype, g)
+    tol = [a + b for a, b in zip(tol, gradual(q, k, v, g, seen, D ** -0.5, dtype))]
+    qd, kd, vd, gd = (to_dev(t) for t in (q, k, v, g))
+    fd = None if first is None else f.to(DEV)
+    p = None if Lq == Lk else pos.to(DEV)
+    o, lse, res = sink_window_attention_fwd(qd, kd, vd, W, S, D ** -0.5, p, fd,
+                                            return_residual=True)
+    close(o.transpose(1, 2), ref[0], tol[0], "o")
+    close(lse, ref[1], tol[1], "lse")
+    grads = sink_window_attention_bwd(qd, kd, vd, o, lse, gd.transpose(1, 2), W, S, D ** -0.5, p,
+                                      fd, res)
+    for got, r, t, what in zip(grads, ref[2:], tol[2:], ("dq", "dk", "dv")):
+        close(got, r, t, what)
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_random_calls(seed):
+    case = random_case(seed)
+    print(case, flush=True)
+    run_case(*case, seed)
+
+
+def test_gradients_of_gradients_and_other_devices_are_refused():
+    layer = SinkWindowAttention(2, 64, 8)
+    q = torch.randn(1, 2, 5, 64, dtype=BF16, device=DEV, requires_grad=True)
+    (g,) = torch.autograd.grad(layer(q, q, q)[0].float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.float().square().sum().backward()
+    q = q.detach()
+    o, lse = sink_window_attention_fwd(q, q, q, 8, 0, 0.125)
+    for bad in ((o.cpu(), lse, o), (o, lse.cpu(), o), (o, lse, o.cpu())):
+        with pytest.raises((RuntimeError, ValueError)):
+            sink_window_attention_bwd(q, q, q, *bad, 8, 0, 0.125)
