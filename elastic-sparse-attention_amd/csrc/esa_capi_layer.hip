@@ -178,13 +178,6 @@ void sink_pattern(SinkArgs& g, const esa_window* w) {
   g.nqb = (g.q_len + 127) / 128;
 }
 
-// Workgroups of the forward that the chip runs at a time, and of dK / dV's kernel
-// (as many a CU as its registers hold)
-int64_t sink_fwd_slots(const SinkArgs& g) {
-  return 256 * (g.elem == ESA_F32 ? (g.d_real > 64 ? 1 : 2) : g.d_real > 64 ? 2 : 4);
-}
-int64_t sink_kv_slots(const SinkArgs& g) { return g.elem == ESA_F32 && g.d_real > 64 ? 256 : 512; }
-
 // Keys that a call's rows walk, at most.
 int64_t sink_keys(const SinkArgs& g) {
   return std::min<int64_t>(g.kv_len, (int64_t)g.window + g.sinks + g.q_len);
@@ -193,24 +186,28 @@ int64_t sink_keys(const SinkArgs& g) {
 // Few rows against many keys take the decode kernel (row tiles of 16 over the
 // heads that share a kv head, the keys cut into ranges side by side), others
 // the forward's 128-row blocks, which walk their keys one after the other.
-// Both estimated: a block walks a key in 0.022 us (float32: 0.08), blocks past
-// the chip's 512 (256) wait for a round; the decode kernel does 13500 (tile,
-// key) pairs a microsecond at head_dim 128, twice that at 64 (float32: 2500,
-// 5000), after 8 us.  Measured, decode against blocks: bf16, head_dim 128, 32
-// heads on 8, window 4096, one sequence, 1 / 16 / 64 rows 13 / 16 / 36 us
-// against 91 / 92 / 94; 8 sequences, 4 / 16 / 32 rows 33 / 95 / 152 against
-// 108 / 115 / 104; 64 sequences, window 1024, 4 / 8 / 16 / 32 rows 55 / 81 /
-// 154 / 302 against 142 / 143 / 144 / 144; float32, head_dim 64, 64 rows 28
-// against 91.
+// Both estimated: a block walks a key in 0.026 us (float32: 0.08, at head_dim
+// past 64 0.14), blocks past the chip's slots wait for a round; the decode
+// kernel does 27000 (tile, key) pairs a microsecond at head_dim 64, 13500 at
+// 128 (float32: 13000, 4900), after 8 us.  Measured, decode against blocks:
+// bf16, head_dim 128, 32 heads on 8, window 4096, one sequence, 1 / 16 / 64
+// rows 13 / 17 / 37 us against 94 / 96 / 99; 8 sequences, 4 / 16 / 32 rows 33 /
+// 96 / 153 against 107 / 107 / 108; 64 sequences, window 1024, 8 / 16 / 32 rows
+// 82 / 157 / 306 against 149 / 147 / 147; head_dim 64, 64 sequences, 8 / 16 rows
+// 46 / 84 against 58 / 59; float32, 16 sequences, 16 heads on 4 of 64, window
+// 2048, 16 / 32 / 64 rows 67 / 83 / 134 against 160 / 161 / 170; 8 sequences, 8
+// heads on 2 of 128, window 1024, 64 rows 57 against 162.
 bool sink_decodes(const SinkArgs& g) {
   if ((int64_t)g.B * g.H * g.q_len >= kMaxGrid / 4) return false;
-  const bool f32 = g.elem == ESA_F32;
+  const bool f32 = g.elem == ESA_F32, narrow = g.d_real <= 64;
   const double keys = (double)sink_keys(g);
   const double tiles = (double)g.B * g.Hkv * (((int64_t)g.groups * g.q_len + 15) / 16);
-  const int64_t blocks = (int64_t)g.B * g.H * g.nqb, slots = sink_fwd_slots(g);
-  const double rate = (f32 ? 2500.0 : 13500.0) * (g.d_real <= 64 ? 2.0 : 1.0);
-  return tiles * keys / rate + 8.0 < keys * (f32 ? 0.08 : 0.022) * (double)((blocks + slots - 1) / slots)
-         || (int64_t)g.groups * g.q_len <= 16;
+  const int64_t blocks = (int64_t)g.B * g.H * g.nqb;
+  const int64_t slots = f32 ? (narrow ? 512 : 256) : narrow ? 768 : 512;
+  const double rate = f32 ? (narrow ? 13000.0 : 4900.0) : narrow ? 27000.0 : 13500.0;
+  const double walk = f32 ? (narrow ? 0.08 : 0.14) : 0.026;
+  return tiles * keys / rate + 8.0 < keys * walk * (double)((blocks + slots - 1) / slots) ||
+         (int64_t)g.groups * g.q_len <= 16;
 }
 
 // Key ranges a row tile: as many as make 512 workgroups (two a CU: with 1024
@@ -274,7 +271,7 @@ int sink_qpad(int q_len) { return (q_len + 3) / 4 * 4; }
 void sink_bwd_plan(SinkArgs& g) {
   g.nkb = (g.kv_len + 127) / 128;
   g.qpad = sink_qpad(g.q_len);
-  const int64_t slots = sink_kv_slots(g), part = g.elem == ESA_F32 ? 1 : 6;
+  const int64_t slots = g.elem == ESA_F32 && g.d_real > 64 ? 256 : 512, part = g.elem == ESA_F32 ? 1 : 6;
   const int64_t kv = (int64_t)g.B * g.Hkv;
   const int n_sink = std::min(g.nkb, (g.sinks + 127) / 128);
   auto stages = [&](int64_t rows) { return (rows + 63) / 64 * g.groups; };
