@@ -3,13 +3,24 @@
 //   s = scale q k^T on visible keys,  o = softmax(s) v,  lse = log sum exp(s)
 //
 // One workgroup (4 waves) takes 128 rows of one (sequence, head) and walks
-// the keys they see: the sinks' blocks, then the window's, or one run of
-// blocks where the two meet.  Each wave holds 32 rows: Q in registers, O^T in
+// the keys they see: the sinks' stages, then the window's, or one run of
+// stages where the two meet.  Each wave holds 32 rows: Q in registers, O^T in
 // accumulators, the running maximum and sum of each row in its lane.  K and V
-// come in stages copied HBM -> LDS without registers, one stage ahead.  A
-// 32 x 32 block costs two products, S^T = K Q^T and O^T += V^T P^T, with P
-// straight from the accumulators; a block of which a wave sees nothing is
-// skipped, one that it sees whole takes no mask.
+// come in stages of 32 keys copied HBM -> LDS without registers, up to two
+// stages ahead.  A 32 x 32 block costs two products, S^T = K Q^T and
+// O^T += V^T P^T, with P straight from the accumulators; a stage of which a
+// wave sees nothing is skipped, one that it sees whole takes no mask.
+//
+// Bound: the vector instructions of a block (about 92 beside its 16 matrix
+// instructions at head_dim 128; a SIMD's vector and matrix pipes overlap in
+// part only: 8 float32 fma after each of two waves' products cost 33% of the
+// products' time on top, 4 nothing), so waves are what counts: with registers
+// for three a SIMD (168, reads' addresses formed anew, three stages in LDS)
+// instead of two, 32768 rows of 32 heads on 8, window 4096, bf16, take 2.02 ms
+// (1020 TFLOP/s) instead of 2.13; operands read 2, 3 or 4 products ahead 2.03,
+// 2.02, 2.05 ms.  8192 rows, window 1024, with o's residual: 180 us; 8 padded
+// sequences of 4099, 16 heads of 64, window 500, f16 (four waves): 130 us,
+// against 149 with three.
 #include "esa_sink.hpp"
 
 namespace esa {
@@ -19,17 +30,17 @@ namespace {
 template <int D, Elem E>
 struct SinkFwdCfg {
   static constexpr int WAVES_PER_SIMD =
-      E == Elem::f32 ? (D >= 128 ? 1 : 2) : D >= 128 ? 2 : 4;
+      E == Elem::f32 ? (D >= 128 ? 1 : 2) : D >= 128 ? 3 : 4;
 };
 
 template <int D, Elem E>
 __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_fwd_kernel(
     SinkArgs A) {
-  using T = SinkTile<D, E>;
+  using T = SinkTile<D, E, true>;
   using Stage = SinkStage<D, E, 32, 256>;
   using LdsT = typename T::LdsT;
   constexpr int ND = T::ND, N = 32 * D;
-  // four stages of 32 keys; separate objects, so that reads of one are seen
+  // three stages of 32 keys; separate objects, so that reads of one are seen
   // not to depend on the copies into another
   __shared__ __attribute__((aligned(1024))) LdsT k0_[N];
   __shared__ __attribute__((aligned(1024))) LdsT v0_[N];
@@ -37,8 +48,6 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
   __shared__ __attribute__((aligned(1024))) LdsT v1_[N];
   __shared__ __attribute__((aligned(1024))) LdsT k2_[N];
   __shared__ __attribute__((aligned(1024))) LdsT v2_[N];
-  __shared__ __attribute__((aligned(1024))) LdsT k3_[N];
-  __shared__ __attribute__((aligned(1024))) LdsT v3_[N];
 
   const RowItem it = row_item(A);
   const int b = it.b, h = it.h, kvh = it.kvh, r0 = it.qb * 128;
@@ -129,52 +138,56 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
     // (past the wave's last key the product is of whatever the buffer holds,
     // and dropped: no branch splits the scores from the softmax)
     if constexpr (T::ES == 2) {
-      // in written order: products and exponentials side by side, V's reads
-      // ahead of the products that take them
-      typename T::V8 ka[T::NS];
-#pragma unroll
-      for (int k = 0; k < T::NS; ++k) ka[k] = t.row_operand(kbuf, 0, k);
-      u32x4 va[ND][2];
+      // In written order, each operand read AHEAD products ahead: the first half
+      // of the scores beside the first half of the exponentials, the second half
+      // of both beside the first products with V, then V's rest.
+      constexpr int AHEAD = 3, NS = T::NS, H = NS / 2, PER = 8 / NS;
+      typename T::V8 ka[NS];
+      u32x4 va[2 * ND];
       typename T::P pp;
-      auto exps = [&](int q) __attribute__((always_inline)) {  // two of the 16
-        s[2 * q] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * q], scale, -m_use));
-        s[2 * q + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * q + 1], scale, -m_use));
-        l_run += s[2 * q] + s[2 * q + 1];
-        asm volatile("" : "+v"(l_run));  // summed here, not behind the last product
-        pp.w[q] = T::M::pack2(s[2 * q], s[2 * q + 1]);
+      int base, vbase;  // of the reads' addresses
+      // product i is of scores (its number) or, from there on, with V
+      auto order = [](int i) constexpr {
+        return i < H ? i : i >= H + NS ? NS + i - NS : (i - H) % 2 ? NS + (i - H) / 2 : (i + H) / 2;
       };
-      constexpr int H = T::NS / 2, EH = 4 / H > 0 ? 4 / H : 1;  // exponential pairs a product
+      auto read = [&](int i) __attribute__((always_inline)) {
+        if (i >= 2 * NS) return;
+        const int o = order(i), k = o % NS;
+        if (o == 0) base = T::fresh(t.ra[0]);
+        if (o == NS) vbase = T::fresh(t.ca[0]);
+        if (o < NS)
+          ka[k] = t.row_operand(kbuf, 0, k, base);
+        else
+          va[k] = t.col_operand(vbuf, 0, k % ND, k / ND, vbase);
+      };
+      auto exps = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
-      for (int k = 0; k < H; ++k) {
-        __builtin_amdgcn_sched_barrier(0);
-        sn = T::M::mfma32(ka[k], qf.f[k], sn);
-        if (k < ND) va[k][0] = t.col_operand(vbuf, 0, k, 0);
-#pragma unroll
-        for (int e = 0; e < EH; ++e) exps(k * EH + e);
-      }
-#pragma unroll
-      for (int k = 0; k < H; ++k) {
-        __builtin_amdgcn_sched_barrier(0);
-        sn = T::M::mfma32(ka[H + k], qf.f[H + k], sn);
-        if (k < ND) va[k][1] = t.col_operand(vbuf, 0, k, 1);
-#pragma unroll
-        for (int e = 0; e < EH; ++e) {
-          exps(4 + k * EH + e);
-          if (e == 0 && k < ND) t.col_step(oacc[k], va[k][0], pp, 0);
+        for (int q = k * PER; q < (k + 1) * PER; ++q) {
+          s[2 * q] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * q], scale, -m_use));
+          s[2 * q + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * q + 1], scale, -m_use));
+          l_run += s[2 * q] + s[2 * q + 1];
+          pp.w[q] = T::M::pack2(s[2 * q], s[2 * q + 1]);
         }
-      }
-      // O is normalised by the probabilities that its product used
+        asm volatile("" : "+v"(l_run));  // summed here, not behind the last product
+      };
 #pragma unroll
-      for (int k = 0; k < ND; ++k) {
+      for (int i = 0; i < AHEAD; ++i) read(i);
+#pragma unroll
+      for (int i = 0; i < 2 * NS; ++i) {
         __builtin_amdgcn_sched_barrier(0);
-        t.col_step(oacc[k], va[k][1], pp, 1);
-        n_run = T::M::dot2(pp.w[2 * k], n_run);
-        n_run = T::M::dot2(pp.w[2 * k + 1], n_run);
-        if (ND == 2) {
-          n_run = T::M::dot2(pp.w[2 * k + 4], n_run);
-          n_run = T::M::dot2(pp.w[2 * k + 5], n_run);
+        const int o = order(i), k = o % NS;
+        if (o < NS) {
+          sn = T::M::mfma32(ka[k], qf.f[k], sn);
+          exps(k);
+        } else {
+          T::col_step(oacc[k % ND], va[k], pp, k / ND);
+          // O is normalised by the probabilities that its product used
+#pragma unroll
+          for (int w = 0; w < PER; ++w)
+            n_run = T::M::dot2(pp.w[4 * (k / ND) + PER * (k % ND) + w], n_run);
+          asm volatile("" : "+v"(n_run));
         }
-        asm volatile("" : "+v"(n_run));
+        read(i + AHEAD);
       }
       top = row_top(sn);
       __builtin_amdgcn_sched_barrier(0);
@@ -193,11 +206,11 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
     s = sn;
     used = next;
   };
-  // stage i's wait: its own loads and the next stage's have landed for every
-  // wave; the one after may be on its way
+  // Stage i's wait, for every wave: its V and the next stage's K have landed
+  // (the next V, issued last, may be on its way)
   auto ready = [&](int i) __attribute__((always_inline)) {
-    if (i + 2 < n_all)
-      stage_wait<2 * Stage::LOADS>();
+    if (i + 1 < n_all)
+      stage_wait<Stage::LOADS>();
     else
       stage_wait<0>();
   };
@@ -209,10 +222,9 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
   };
   issue(0, k0_, v0_);
   issue(1, k1_, v1_);
-  issue(2, k2_, v2_);
   if (n_all > 0) {
-    if (n_all > 2)
-      stage_wait<4 * Stage::LOADS>();
+    if (n_all > 1)
+      stage_wait<3 * Stage::LOADS>();
     else
       stage_wait<0>();
     if (ws.sees(0)) {
@@ -222,22 +234,18 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
       used = true;
     }
   }
-  for (int i = 0; i < n_all; i += 4) {
+  for (int i = 0; i < n_all; i += 3) {
     ready(i);
-    issue(i + 3, k3_, v3_);
+    issue(i + 2, k2_, v2_);
     step(v0_, k1_, i);
     if (i + 1 >= n_all) break;
     ready(i + 1);
-    issue(i + 4, k0_, v0_);
+    issue(i + 3, k0_, v0_);
     step(v1_, k2_, i + 1);
     if (i + 2 >= n_all) break;
     ready(i + 2);
-    issue(i + 5, k1_, v1_);
-    step(v2_, k3_, i + 2);
-    if (i + 3 >= n_all) break;
-    ready(i + 3);
-    issue(i + 6, k2_, v2_);
-    step(v3_, k0_, i + 3);
+    issue(i + 4, k1_, v1_);
+    step(v2_, k0_, i + 2);
   }
 
   // ---- O rows and log-sum-exp
