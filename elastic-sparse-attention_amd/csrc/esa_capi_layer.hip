@@ -259,13 +259,13 @@ int sink_qpad(int q_len) { return (q_len + 3) / 4 * 4; }
 // How the rows of a kv head's key blocks are cut, in stages of 64 rows and
 // heads.  The chip runs `slots` blocks at a time; a chunk costs what its stages
 // do and about `part` stages more for its float32 part (written, read and
-// joined).  Counted so, with the blocks alike (a window):
+// joined; one where float32 products make a stage itself as long).  Counted so, with the blocks alike (a window):
 //   a sinks' block is cut into pieces of a window block's size;
 //   of all blocks the whole rounds stay whole, and those that would run as an
 //   unfilled last round (or all of a grid too small for one) are cut so that
 //   they fill it together (8192 rows, 8 kv heads of 4 query heads, window 1024
 //   and 4 sinks, head_dim 128: 568 blocks on 512 slots, two rounds of 72 stages
-//   against one and a fifth: 480 us, 365);
+//   against one and a fifth: 480 us and 365, before the kernel itself was faster);
 // where the first blocks see many more rows than the last (a window near the
 // sequence's length) all are cut alike, to at most 2/3 of a slot's share.
 void sink_bwd_plan(SinkArgs& g) {

@@ -20,7 +20,10 @@
 // pair, shared by all heads; tables would be read from HBM) and stay in
 // registers while the lanes go through its heads, the next head's row on its
 // way.  A pair's other half comes from its lane by a DPP rotation (16 lanes a
-// row) or a shuffle.
+// row) or a shuffle.  32768 tokens of 32 + 8 heads of 128, bf16, views of one
+// projection: 169 us, 3.97 TB/s (a copy of as much: 137 us at 4.89; with a row's
+// lanes going from token to token of one head 187, tables read again for each);
+// 15003 tokens of 16 + 4 heads of 96, f16: forward 26 (41), backward 45 (58).
 #include "esa_rotary.hpp"
 #include "esa_mma.hpp"
 

@@ -117,13 +117,13 @@ inline int sink_xcd_runs(const SinkArgs& a, int64_t grid) {
   return ((int64_t)a.B * a.Hkv) % 8 == 0 && grid % 8 == 0;
 }
 
-// The key stages of 128 rows from r0: n_sink stages of the sinks, then stages
-// from m0 to the last row's position; one run where the two meet.
+// The key stages (32 keys) of 128 rows from r0: n_sink stages of the sinks, then
+// stages from m0 to the last row's position; one run where the two meet.
 struct KeyStages {
-  int f, n_sink, m0, n_all, step;
+  int f, n_sink, m0, n_all;
   int pb;  // the last row's position, inside the cache
   __device__ __forceinline__ int key0(int i) const {
-    return i < n_sink ? f + i * step : m0 + (i - n_sink) * step;
+    return i < n_sink ? f + i * 32 : m0 + (i - n_sink) * 32;
   }
 };
 // What the rows [p0, p0 + 31] of one wave (its last one p1, no row: p1 < p0)
@@ -137,36 +137,32 @@ struct WaveStages {
   }
   __device__ __forceinline__ bool full(int i) const { return (uint32_t)(i - full_lo) < (uint32_t)full_n; }
 };
-template <int STAGE>
 __device__ __forceinline__ WaveStages wave_stages(const KeyStages& k, int p0, int p1, int window,
                                                   int sink_end) {
-  auto floor_div = [](int a) { return a >> (STAGE == 64 ? 6 : 5); };
-  static_assert(STAGE == 64 || STAGE == 32, "stage");
+  auto floor_div = [](int a) { return a >> 5; };
   WaveStages w;
-  // k0 <= p1;  k0 + STAGE - 1 > p0 - window;  k0 < sink_end
+  // k0 <= p1;  k0 + 31 > p0 - window;  k0 < sink_end
   w.last = p1 < p0 ? -1 : k.n_sink + max(floor_div(p1 - k.m0), -1);
   w.first = k.n_sink + floor_div(max(p0 - window + 1 - k.m0, 0));
   w.sinks = k.n_sink + (sink_end > k.m0 ? floor_div(sink_end - 1 - k.m0) + 1 : 0);
-  // k0 > p0 + 31 - window and k0 + STAGE - 1 <= p0
+  // k0 > p0 + 31 - window and k0 + 31 <= p0
   w.full_lo = k.n_sink + max(floor_div(p0 + 31 - window - k.m0) + 1, 0);
   w.full_n = max(k.n_sink + floor_div(p0 + 1 - k.m0) - w.full_lo, 0);
   return w;
 }
-template <int STAGE>
 __device__ __forceinline__ KeyStages key_stages(const SinkArgs& A, const SeqInfo& si, int r0,
                                                 int sink_end) {
   KeyStages k;
-  k.step = STAGE;
   k.f = si.first;
   k.pb = min(si.base + min(r0 + 127, A.q_len - 1), A.kv_len - 1);
   const int lo = max(k.f, si.base + r0 - A.window + 1);
-  k.n_sink = lo > k.f && k.pb >= k.f ? (min(sink_end, lo) - k.f + STAGE - 1) / STAGE : 0;
+  k.n_sink = lo > k.f && k.pb >= k.f ? (min(sink_end, lo) - k.f + 31) / 32 : 0;
   k.m0 = lo;
-  if (k.n_sink > 0 && lo <= k.f + k.n_sink * STAGE) {
+  if (k.n_sink > 0 && lo <= k.f + k.n_sink * 32) {
     k.n_sink = 0;
     k.m0 = k.f;
   }
-  k.n_all = k.n_sink + (k.pb >= k.m0 ? (k.pb - k.m0) / STAGE + 1 : 0);
+  k.n_all = k.n_sink + (k.pb >= k.m0 ? (k.pb - k.m0) / 32 + 1 : 0);
   return k;
 }
 

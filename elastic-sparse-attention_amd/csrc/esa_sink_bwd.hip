@@ -11,11 +11,11 @@
 //                     where the forward kept the difference: a rounded O alone
 //                     leaves dQ and dK about 8% further off) and lse in log2
 //                     units, left for the next kernel (a kernel of its own for
-//                     them read dO once more: 37 us against 28
-//                     more here, 8192 rows of 32 heads of 128)
+//                     them read dO once more: 37 us, here 28 more, for 8192
+//                     rows of 32 heads of 128)
 //   sink_dkdv_kernel  128 keys a workgroup, over the rows that see them: the
-//                     lane's own key row (K, V) in registers, rows of Q and dO
-//                     staged in LDS: S = Q K^T, dP = dO V^T, dV^T += dO^T P,
+//                     lane's own key row (K, V) in registers (or V in LDS), rows
+//                     of Q and dO staged in LDS: S = Q K^T, dP = dO V^T, dV^T += dO^T P,
 //                     dK^T += Q^T dS
 //   sink_join_kernel  blocks whose rows were split: the parts in order
 //
@@ -24,6 +24,18 @@
 // after the other, and may be cut into chunks, one workgroup each, that leave
 // float32 parts: a sink's block, which every later row sees, and the blocks
 // that would run as an unfilled last round of the grid (sink_bwd_plan).
+//
+// Bound: registers, and with them waves: dK, dV and K of 32 keys take 160 of a
+// wave's 256 at head_dim 128, so two waves a SIMD share its pipes and wait for
+// each other's products (of dK / dV's cycles the matrix pipe works 50%, of
+// dQ's 42%).  V in LDS leaves dK / dV room to read each operand three products
+// ahead and to place the exponentials and dS beside products: with V in
+// registers and one product after the other 365 us, so 275 (8192 rows, 32 heads
+// on 8, window 1024, bf16: 930 TFLOP/s of its four products); dQ, a pipeline of
+// 32-key stages as the forward, 240 against 262 with 64-key stages and no
+// pipeline (700 TFLOP/s of its three), 20 of it the rows' delta.  8 padded
+// sequences of 4099, 16 heads of 64, window 500, f16: 194 and 167; float32, 2 x
+// 2048 rows, 8 heads of 64, window 256: 100 (114 with one wave a SIMD) and 55.
 #include <algorithm>
 
 #include "esa_sink.hpp"
@@ -112,7 +124,7 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::DQ_WAVES)) void sink_dq_ker
   const int b = it.b, h = it.h, kvh = it.kvh, r0 = it.qb * 128;
   const SeqInfo si = seq_info(A, b);
   const int f = si.first, sink_end = min(f + A.sinks, A.kv_len), W = A.window;
-  const KeyStages keys = key_stages<32>(A, si, r0, sink_end);
+  const KeyStages keys = key_stages(A, si, r0, sink_end);
 
   const int tid = threadIdx.x;
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -122,7 +134,7 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::DQ_WAVES)) void sink_dq_ker
   const int p = si.base + r;
   const int pb = keys.pb, pw0 = si.base + r0 + wave * 32, pw1 = min(pw0 + 31, pb);
   const int n_all = keys.n_all;
-  const WaveStages ws = wave_stages<32>(keys, pw0, pw1, W, sink_end);
+  const WaveStages ws = wave_stages(keys, pw0, pw1, W, sink_end);
 
   Stage ks, vs;
   ks.init(at<E>(A.k, (int64_t)b * A.ksb + (int64_t)kvh * A.ksh), A.kss, A.kv_len, A.d_real, tid);

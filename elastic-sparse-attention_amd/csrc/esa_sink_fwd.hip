@@ -53,7 +53,7 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
   const int b = it.b, h = it.h, kvh = it.kvh, r0 = it.qb * 128;
   const SeqInfo si = seq_info(A, b);
   const int f = si.first, sink_end = min(f + A.sinks, A.kv_len), W = A.window;
-  const KeyStages keys = key_stages<32>(A, si, r0, sink_end);
+  const KeyStages keys = key_stages(A, si, r0, sink_end);
 
   const int tid = threadIdx.x;
   const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -63,7 +63,7 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
   const int p = si.base + r;
   const int pb = keys.pb, pw0 = si.base + r0 + wave * 32, pw1 = min(pw0 + 31, pb);
   const int n_all = keys.n_all;
-  const WaveStages ws = wave_stages<32>(keys, pw0, pw1, W, sink_end);
+  const WaveStages ws = wave_stages(keys, pw0, pw1, W, sink_end);
 
   T t;
   t.init(lane);
