@@ -257,7 +257,9 @@ esa_status sink_fwd_shape(const esa_fwd_args* a, const esa_window* w) {
 int sink_qpad(int q_len) { return (q_len + 3) / 4 * 4; }
 
 // How the rows of a kv head's key blocks are cut, in stages of 64 rows and
-// heads.  The chip runs `slots` blocks at a time; a chunk costs what its stages
+// heads.  The chip runs `slots` blocks at a time (two a CU; float32 products
+// leave a CU nothing for a second: 2 x 2048 rows, 8 heads of 64, window 256, 336
+// blocks counted on 256 slots 76 us, on 512 100); a chunk costs what its stages
 // do and about `part` stages more for its float32 part (written, read and
 // joined; one where float32 products make a stage itself as long).  Counted so, with the blocks alike (a window):
 //   a sinks' block is cut into pieces of a window block's size;
@@ -271,7 +273,7 @@ int sink_qpad(int q_len) { return (q_len + 3) / 4 * 4; }
 void sink_bwd_plan(SinkArgs& g) {
   g.nkb = (g.kv_len + 127) / 128;
   g.qpad = sink_qpad(g.q_len);
-  const int64_t slots = g.elem == ESA_F32 && g.d_real > 64 ? 256 : 512, part = g.elem == ESA_F32 ? 1 : 6;
+  const int64_t slots = g.elem == ESA_F32 ? 256 : 512, part = g.elem == ESA_F32 ? 1 : 6;
   const int64_t kv = (int64_t)g.B * g.Hkv;
   const int n_sink = std::min(g.nkb, (g.sinks + 127) / 128);
   auto stages = [&](int64_t rows) { return (rows + 63) / 64 * g.groups; };

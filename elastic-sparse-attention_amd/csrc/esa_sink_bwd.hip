@@ -35,7 +35,8 @@
 // 32-key stages as the forward, 240 against 262 with 64-key stages and no
 // pipeline (700 TFLOP/s of its three), 20 of it the rows' delta.  8 padded
 // sequences of 4099, 16 heads of 64, window 500, f16: 194 and 167; float32, 2 x
-// 2048 rows, 8 heads of 64, window 256: 100 (114 with one wave a SIMD) and 55.
+// 2048 rows, 8 heads of 64, window 256: 76 (and 100 against 114 with one wave a
+// SIMD, before its grid was cut for 256 slots) and 54.
 #include <algorithm>
 
 #include "esa_sink.hpp"
