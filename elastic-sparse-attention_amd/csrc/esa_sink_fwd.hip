@@ -16,11 +16,12 @@
 // part only: 8 float32 fma after each of two waves' products cost 33% of the
 // products' time on top, 4 nothing), so waves are what counts: with registers
 // for three a SIMD (168, reads' addresses formed anew, three stages in LDS)
-// instead of two, 32768 rows of 32 heads on 8, window 4096, bf16, take 2.02 ms
-// (1020 TFLOP/s) instead of 2.13; operands read 2, 3 or 4 products ahead 2.03,
-// 2.02, 2.05 ms.  8192 rows, window 1024, with o's residual: 180 us; 8 padded
-// sequences of 4099, 16 heads of 64, window 500, f16 (four waves): 130 us,
-// against 149 with three.
+// instead of two, 32768 rows of 32 heads on 8, window 4096, bf16, take 2.11 ms
+// (980 TFLOP/s) instead of 2.17 on one card (2.02 on another), though a grid
+// that is one round of two blocks a CU gains no wave: 2048 such rows 158 us
+// instead of 152.  Operands read 2, 3 or 4 products ahead: 2.03, 2.02, 2.05 ms.
+// 8192 rows, window 1024, with o's residual: 180 us; 8 padded sequences of 4099,
+// 16 heads of 64, window 500, f16 (four waves): 130 us, against 149 with three.
 #include "esa_sink.hpp"
 
 namespace esa {
