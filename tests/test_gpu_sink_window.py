@@ -590,3 +590,55 @@ def test_gradients_of_gradients_and_other_devices_are_refused():
     for bad in ((o.cpu(), lse, o), (o, lse.cpu(), o), (o, lse, o.cpu())):
         with pytest.raises((RuntimeError, ValueError)):
             sink_window_attention_bwd(q, q, q, *bad, 8, 0, 0.125)
+
+
+@pytest.mark.parametrize("dtype,D", [(BF16, 128), (F16, 64), (F32, 64)])
+def test_broadcast_inputs(dtype, D):
+    """One key and value row set for every sequence and head, one query row set
+    for every sequence: the calls see views of stride 0, as their copies."""
+    B, H, Hkv, L = 3, 4, 2, 150
+    gen = torch.Generator().manual_seed(21)
+    q1 = torch.randn(1, H, L, D, generator=gen).to(dtype).to(DEV).requires_grad_()
+    k1 = torch.randn(1, 1, L, D, generator=gen).to(dtype).to(DEV).requires_grad_()
+    v1 = torch.randn(B, Hkv, 1, D, generator=gen).to(dtype).to(DEV).requires_grad_()
+    g = torch.randn(B, L, H * D, generator=gen).to(dtype).to(DEV)
+    layer = SinkWindowAttention(H, D, 40, 3, Hkv)
+
+    def grads(copy):
+        q, k, v = (t.expand(B, h, L, D) for t, h in ((q1, H), (k1, Hkv), (v1, Hkv)))
+        if copy:
+            q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+        o = layer(q, k, v)[0]
+        return (o.detach(), *torch.autograd.grad(o, (q1, k1, v1), g))
+
+    for a, b in zip(grads(False), grads(True)):
+        assert a.shape == b.shape and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("B,H,Hkv,Lq,Lk", [(4100, 8, 1, 1, 3), (1, 600, 3, 1, 40), (1, 70, 70, 2, 2),
+                                           (2000, 2, 2, 3, 3)])
+def test_many_sequences_and_heads(B, H, Hkv, Lq, Lk):
+    D, W, S = 64, 3, 1
+    gen = torch.Generator().manual_seed(22)
+    q, k, v = (torch.randn(B, h, n, D, generator=gen).to(BF16)
+               for h, n in ((H, Lq), (Hkv, Lk), (Hkv, Lk)))
+    pos = (Lk - Lq + torch.arange(Lq)).expand(B, Lq)
+    seen = window_mask(pos, torch.zeros(B, dtype=torch.int64), Lk, W, S)
+    ref, tol = bounds(q, k, v, seen, D ** -0.5, BF16)
+    rotary = QKNormRope(D).to(DEV).to(BF16)
+    qd, kd, vd = q.to(DEV), k.to(DEV), v.to(DEV)
+    o, lse = sink_window_attention_fwd(qd, kd, vd, W, S, D ** -0.5, pos.to(DEV))
+    close(o.transpose(1, 2), ref[0], tol[0], "o")
+    close(lse, ref[1], tol[1], "lse")
+    # the whole step, against the rotation and the attention by themselves
+    layer = SinkWindowAttention(H, D, W, S, Hkv, rotary=rotary)
+    caches = torch.zeros_like(kd), torch.zeros_like(vd)
+    with torch.no_grad():
+        got = layer(qd, kd[:, :, -Lq:], vd[:, :, -Lq:], cache_position=pos.to(DEV),
+                    kv_cache=caches)[0]
+        yq, yk = rotary(qd, kd[:, :, -Lq:], pos.to(DEV))
+    want_k, want_v = torch.zeros_like(kd), torch.zeros_like(vd)
+    want_k[:, :, -Lq:], want_v[:, :, -Lq:] = yk, vd[:, :, -Lq:]
+    assert torch.equal(caches[0], want_k) and torch.equal(caches[1], want_v)
+    want, _ = sink_window_attention_fwd(yq, want_k, want_v, W, S, D ** -0.5, pos.to(DEV))
+    assert torch.equal(got, want.view(B, Lq, H * D))
