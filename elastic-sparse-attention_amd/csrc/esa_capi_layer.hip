@@ -55,10 +55,19 @@ void rotary_grid(RotaryArgs& g, int batch, bool append, bool bwd) {
   g.lanes = 8;
   while (g.lanes * g.vec < g.D) g.lanes *= 2;
   const int tok = 256 / g.lanes;
+  // Where a token's heads are side by side in memory and the rows do not fit the
+  // 256 MiB last-level cache, two lane groups take two heads of a token instead
+  // of one of two tokens: twice the bytes at an address (40 heads of 128, bf16,
+  // views of one projection, one and two: 32768 tokens 171 and 160 us, 16384 82
+  // and 78, but 4096 26 and 27; the backward's five streams gain nothing, 256
+  // and 271).
+  const int es = g.elem == ESA_F32 ? 4 : 2;
+  g.side = !bwd && g.qsh < g.qss && g.ksh < g.kss &&
+                   2 * es * (double)batch * g.n * g.heads * g.D > double(256 << 20) ? 2 : 1;
   g.tokens = batch * g.n;
   g.n_tiles = (int)(((int64_t)g.tokens + tok - 1) / tok);
   const int64_t split = std::min<int64_t>(g.heads, (511 + g.n_tiles) / g.n_tiles);
-  g.heads_per_split = (int)((g.heads + split - 1) / split);
+  g.heads_per_split = ((int)((g.heads + split - 1) / split) + g.side - 1) / g.side * g.side;
   g.n_splits = (g.heads + g.heads_per_split - 1) / g.heads_per_split;
   // (a grid dimension holds fewer than 2^32 work-items: 256 a workgroup)
   g.grid_tiles = std::min(g.n_tiles, bwd ? kRotBwdGrid : 1 << 23);

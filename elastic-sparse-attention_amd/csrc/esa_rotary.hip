@@ -20,10 +20,12 @@
 // pair, shared by all heads; tables would be read from HBM) and stay in
 // registers while the lanes go through its heads, the next head's row on its
 // way.  A pair's other half comes from its lane by a DPP rotation (16 lanes a
-// row) or a shuffle.  32768 tokens of 32 + 8 heads of 128, bf16, views of one
-// projection: 169 us, 3.97 TB/s (a copy of as much: 137 us at 4.89; with a row's
-// lanes going from token to token of one head 187, tables read again for each);
-// 15003 tokens of 16 + 4 heads of 96, f16: forward 26 (41), backward 45 (58).
+// row) or a shuffle.  Rows past the last-level cache whose heads are side by side
+// are taken two heads at a time (SIDE).  32768 tokens of 32 + 8 heads of 128,
+// bf16, views of one projection: 158 us, 4.25 TB/s (a copy of as much: 137 us at
+// 4.89; 171 with one head at a time; 187 with a row's lanes going from token to
+// token of one head, tables read again for each); 15003 tokens of 16 + 4 heads of
+// 96, f16: forward 26 (41), backward 45 (58).
 #include "esa_rotary.hpp"
 #include "esa_mma.hpp"
 
@@ -104,7 +106,8 @@ __device__ __forceinline__ float row_sum(float x) {
   return x;
 }
 
-template <Elem E, int V, int LPR, int MODE>
+// SIDE: heads of a token that lane groups take side by side (1, or 2)
+template <Elem E, int V, int LPR, int MODE, int SIDE>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs A) {
   using T = typename ElemT<E>::T;
   using P = Piece<E, V>;
@@ -113,7 +116,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs A) {
   __shared__ float2 cs[TOK * (LPR * V / 2)];
 
   const int tid = threadIdx.x;
-  const int lane = tid % LPR, sub = tid / LPR;
+  const int lane = tid % LPR, group = tid / LPR;
+  const int hsub = group % SIDE;  // the group's heads: hsub + SIDE i
   const int e0 = lane * V;
   const bool on = e0 < A.D;
   const int half = A.rd / 2;
@@ -154,115 +158,130 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs A) {
       cs[i] = make_float2(c, s);
     }
     __syncthreads();
-    if (sub >= nt) continue;  // (no barrier before the next tile's first one)
-
-    const int64_t b = fast_div((uint32_t)(g0 + sub), A.div_n), s = g0 + sub - b * A.n;
-    int64_t os = s;  // the output's row
-    if constexpr (MODE == kAppend) {
-      // row s of the sequence belongs at base + s inside the cache; any other
-      // position (out of range, repeated, out of order) is written nowhere
-      const int64_t* pos = A.pos + b * A.pos_sb;
-      int64_t base = pos[0], p = pos[s];
-      base += base < 0 ? A.kv_len : 0;
-      p += p < 0 ? A.kv_len : 0;
-      os = base >= 0 && p == base + s && p < A.kv_len ? p : -1;
-    }
-    // y[e] = x[e] c[e] + (the pair's other element) sn[e]
-    float c[V], sn[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      float2 t = make_float2(1.f, 0.f);
-      if (rot) t = cs[sub * half + pair0 + (A.interleaved ? e / 2 : e)];
-      c[e] = t.x;
-      sn[e] = (A.interleaved ? e & 1 : second) ? t.y : -t.y;
-    }
-    auto turn = [&](const float (&x)[V], float (&y)[V], float dir) __attribute__((always_inline)) {
-      if (A.interleaved) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) y[e] = x[e] * c[e] + dir * x[e ^ 1] * sn[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          y[e] = x[e] * c[e] + dir * other_half<LPR>(x[e], partner, across8) * sn[e];
+    // (no barrier before the next tile's first one)
+#pragma unroll 1
+    for (int sub = group / SIDE; sub < nt; sub += TOK / SIDE) {
+      const int64_t b = fast_div((uint32_t)(g0 + sub), A.div_n), s = g0 + sub - b * A.n;
+      int64_t os = s;  // the output's row
+      if constexpr (MODE == kAppend) {
+        // row s of the sequence belongs at base + s inside the cache; any other
+        // position (out of range, repeated, out of order) is written nowhere
+        const int64_t* pos = A.pos + b * A.pos_sb;
+        int64_t base = pos[0], p = pos[s];
+        base += base < 0 ? A.kv_len : 0;
+        p += p < 0 ? A.kv_len : 0;
+        os = base >= 0 && p == base + s && p < A.kv_len ? p : -1;
       }
-      // (elements past rotary_dim as they are: a neighbour's infinity is not theirs)
+      // y[e] = x[e] c[e] + (the pair's other element) sn[e]
+      float c[V], sn[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) y[e] = rot ? y[e] : x[e];
-    };
-    // `count` heads of q or k from src (and g), results to dst (or nowhere)
-    auto heads = [&](const T* src, int64_t sh, const T* g, int64_t gh, T* dst, int64_t dh,
-                     int count, const float (&w)[V], float (&sums)[V], bool lost)
-                     __attribute__((always_inline)) {
-      P in, gin;
-      in.w = gin.w = W{};
-      if (on) in.w = *(const W*)src;
-      if (MODE == kBwd && on) gin.w = *(const W*)g;
-      for (int i = 0; i < count; ++i) {
-        const P xin = in, ggin = gin;
-        src += sh;
-        g += gh;
-        if (i + 1 < count && on) {  // the next head's row, on its way meanwhile
-          in.w = *(const W*)src;
-          if (MODE == kBwd) gin.w = *(const W*)g;
-        }
-        float x[V], y[V], ss = 0.f;
+      for (int e = 0; e < V; ++e) {
+        float2 t = make_float2(1.f, 0.f);
+        if (rot) t = cs[sub * half + pair0 + (A.interleaved ? e / 2 : e)];
+        c[e] = t.x;
+        sn[e] = (A.interleaved ? e & 1 : second) ? t.y : -t.y;
+      }
+      auto turn = [&](const float (&x)[V], float (&y)[V], float dir) __attribute__((always_inline)) {
+        if (A.interleaved) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          x[e] = xin.get(e);
-          ss = __builtin_fmaf(x[e], x[e], ss);
-        }
-        if constexpr (MODE != kBwd) {
-          const float r = rsqrtf(__builtin_fmaf(row_sum<LPR>(ss), inv_d, A.eps));
-#pragma unroll
-          for (int e = 0; e < V; ++e) x[e] *= r * w[e];
-          turn(x, y, 1.f);
-          if (MODE == kAppend && lost) {
-#pragma unroll
-            for (int e = 0; e < V; ++e) y[e] = __builtin_nanf("");
-          }
+          for (int e = 0; e < V; ++e) y[e] = x[e] * c[e] + dir * x[e ^ 1] * sn[e];
         } else {
-          float gr[V], dot = 0.f;
 #pragma unroll
-          for (int e = 0; e < V; ++e) gr[e] = ggin.get(e);
-          turn(gr, y, -1.f);  // the rotation undone
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            gr[e] = y[e] * w[e];
-            dot = __builtin_fmaf(gr[e], x[e], dot);
-          }
-          ss = row_sum<LPR>(ss);
-          dot = row_sum<LPR>(dot);
-          const float r = rsqrtf(__builtin_fmaf(ss, inv_d, A.eps));
-          const float m = dot * inv_d * r * r;  // mean(g gain n) r
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            sums[e] += y[e] * (x[e] * r);
-            y[e] = r * (gr[e] - x[e] * m);
-          }
+          for (int e = 0; e < V; ++e)
+            y[e] = x[e] * c[e] + dir * other_half<LPR>(x[e], partner, across8) * sn[e];
         }
-        if (on) store_piece<E, V>(dst, y);
-        dst += dh;
+        // (elements past rotary_dim as they are: a neighbour's infinity is not theirs)
+#pragma unroll
+        for (int e = 0; e < V; ++e) y[e] = rot ? y[e] : x[e];
+      };
+      // the group's of `n` heads of q or k from src (and g), results to dst
+      auto heads = [&](const T* src, int64_t sh, const T* g, int64_t gh, T* dst, int64_t dh,
+                       int n, const float (&w)[V], float (&sums)[V], bool lost)
+                       __attribute__((always_inline)) {
+        const int count = (n - hsub + SIDE - 1) / SIDE;
+        if (SIDE > 1) {
+          if (count <= 0) return;
+          src += hsub * sh;
+          g += hsub * gh;
+          dst += hsub * dh;
+          sh *= SIDE;
+          gh *= SIDE;
+          dh *= SIDE;
+        }
+        P in, gin;
+        in.w = gin.w = W{};
+        if (on) in.w = *(const W*)src;
+        if (MODE == kBwd && on) gin.w = *(const W*)g;
+        for (int i = 0; i < count; ++i) {
+          const P xin = in, ggin = gin;
+          src += sh;
+          g += gh;
+          if (i + 1 < count && on) {  // the next head's row, on its way meanwhile
+            in.w = *(const W*)src;
+            if (MODE == kBwd) gin.w = *(const W*)g;
+          }
+          float x[V], y[V], ss = 0.f;
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            x[e] = xin.get(e);
+            ss = __builtin_fmaf(x[e], x[e], ss);
+          }
+          if constexpr (MODE != kBwd) {
+            const float r = rsqrtf(__builtin_fmaf(row_sum<LPR>(ss), inv_d, A.eps));
+#pragma unroll
+            for (int e = 0; e < V; ++e) x[e] *= r * w[e];
+            turn(x, y, 1.f);
+            if (MODE == kAppend && lost) {
+#pragma unroll
+              for (int e = 0; e < V; ++e) y[e] = __builtin_nanf("");
+            }
+          } else {
+            float gr[V], dot = 0.f;
+#pragma unroll
+            for (int e = 0; e < V; ++e) gr[e] = ggin.get(e);
+            turn(gr, y, -1.f);  // the rotation undone
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              gr[e] = y[e] * w[e];
+              dot = __builtin_fmaf(gr[e], x[e], dot);
+            }
+            ss = row_sum<LPR>(ss);
+            dot = row_sum<LPR>(dot);
+            const float r = rsqrtf(__builtin_fmaf(ss, inv_d, A.eps));
+            const float m = dot * inv_d * r * r;  // mean(g gain n) r
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              sums[e] += y[e] * (x[e] * r);
+              y[e] = r * (gr[e] - x[e] * m);
+            }
+          }
+          if (on) store_piece<E, V>(dst, y);
+          dst += dh;
+        }
+      };
+      const int nq = min(h1, A.H) - h0;
+      if (nq > 0)
+        heads((const T*)A.q + b * A.qsb + h0 * A.qsh + s * A.qss + e0, A.qsh,
+              (const T*)A.gq + b * A.gqsb + h0 * A.gqsh + s * A.gqss + e0, A.gqsh,
+              (T*)A.qo + b * A.qosb + h0 * A.qosh + s * A.qoss + e0, A.qosh, nq, wq, gq,
+              // a query row with no place in the cache: NaN, as the attention
+              // over the cache gives it
+              MODE == kAppend && os < 0);
+      const int k0 = max(h0 - A.H, 0), nk = min(h1 - A.H, A.Hkv) - k0;
+      if (nk > 0 && os >= 0)
+        heads((const T*)A.k + b * A.ksb + k0 * A.ksh + s * A.kss + e0, A.ksh,
+              (const T*)A.gk + b * A.gksb + k0 * A.gksh + s * A.gkss + e0, A.gksh,
+              (T*)A.ko + b * A.kosb + k0 * A.kosh + os * A.koss + e0, A.kosh, nk, wk, gk, false);
+      if constexpr (MODE == kAppend) {  // values go to their cache as they are
+        const int v0 = max(h0 - A.H - A.Hkv, 0), v1 = h1 - A.H - A.Hkv;
+        const T* src = (const T*)A.v + b * A.vsb + (v0 + hsub) * A.vsh + s * A.vss + e0;
+        T* dst = (T*)A.vo + b * A.vosb + (v0 + hsub) * A.vosh + os * A.voss + e0;
+        for (int h = v0 + hsub; h < v1 && os >= 0 && on; h += SIDE) {
+          *(W*)dst = *(const W*)src;
+          src += SIDE * A.vsh;
+          dst += SIDE * A.vosh;
+        }
       }
-    };
-    const int nq = min(h1, A.H) - h0;
-    if (nq > 0)
-      heads((const T*)A.q + b * A.qsb + h0 * A.qsh + s * A.qss + e0, A.qsh,
-            (const T*)A.gq + b * A.gqsb + h0 * A.gqsh + s * A.gqss + e0, A.gqsh,
-            (T*)A.qo + b * A.qosb + h0 * A.qosh + s * A.qoss + e0, A.qosh, nq, wq, gq,
-            // a query row with no place in the cache: NaN, as the attention
-            // over the cache gives it
-            MODE == kAppend && os < 0);
-    const int k0 = max(h0 - A.H, 0), nk = min(h1 - A.H, A.Hkv) - k0;
-    if (nk > 0 && os >= 0)
-      heads((const T*)A.k + b * A.ksb + k0 * A.ksh + s * A.kss + e0, A.ksh,
-            (const T*)A.gk + b * A.gksb + k0 * A.gksh + s * A.gkss + e0, A.gksh,
-            (T*)A.ko + b * A.kosb + k0 * A.kosh + os * A.koss + e0, A.kosh, nk, wk, gk, false);
-    if constexpr (MODE == kAppend) {  // values go to their cache as they are
-      const int v0 = max(h0 - A.H - A.Hkv, 0), v1 = h1 - A.H - A.Hkv;
-      const T* src = (const T*)A.v + b * A.vsb + v0 * A.vsh + s * A.vss + e0;
-      T* dst = (T*)A.vo + b * A.vosb + v0 * A.vosh + os * A.voss + e0;
-      for (int h = v0; h < v1 && os >= 0 && on; ++h, src += A.vsh, dst += A.vosh)
-        *(W*)dst = *(const W*)src;
     }
   }
 
@@ -275,7 +294,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs A) {
     for (int which = 0; which < 2; ++which) {
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < V; ++e) red[sub * (LPR * V) + e0 + e] = which ? gk[e] : gq[e];
+      for (int e = 0; e < V; ++e) red[group * (LPR * V) + e0 + e] = which ? gk[e] : gq[e];
       __syncthreads();
       for (int d = tid; d < A.D; d += 256) {
         float sum = 0.f;
@@ -309,16 +328,26 @@ __global__ __launch_bounds__(1024) void rotary_gain_kernel(const float* partial,
   }
 }
 
+template <Elem E, int V, int LPR, int MODE>
+void launch_side(const RotaryArgs& a, dim3 grid, hipStream_t stream) {
+  if constexpr (MODE != kBwd)
+    if (a.side == 2) {
+      rotary_kernel<E, V, LPR, MODE, 2><<<grid, 256, 0, stream>>>(a);
+      return;
+    }
+  rotary_kernel<E, V, LPR, MODE, 1><<<grid, 256, 0, stream>>>(a);
+}
+
 template <Elem E, int V, int MODE>
 void launch_lpr(const RotaryArgs& a, dim3 grid, hipStream_t stream) {
   if (a.lanes == 8)
-    rotary_kernel<E, V, 8, MODE><<<grid, 256, 0, stream>>>(a);
+    launch_side<E, V, 8, MODE>(a, grid, stream);
   else if (a.lanes == 16)
-    rotary_kernel<E, V, 16, MODE><<<grid, 256, 0, stream>>>(a);
+    launch_side<E, V, 16, MODE>(a, grid, stream);
   else if (a.lanes == 32)
-    rotary_kernel<E, V, 32, MODE><<<grid, 256, 0, stream>>>(a);
+    launch_side<E, V, 32, MODE>(a, grid, stream);
   else
-    rotary_kernel<E, V, 64, MODE><<<grid, 256, 0, stream>>>(a);
+    launch_side<E, V, 64, MODE>(a, grid, stream);
 }
 
 template <int MODE>

@@ -23,6 +23,7 @@ struct RotaryArgs {
   // the grid: tiles of 256 / (lanes a row) of all sequences' tokens, heads (q, k
   // and, to append, v) in splits; grid_tiles workgroups walk the n_tiles tiles
   int lanes, tokens, n_tiles, grid_tiles;
+  int side;  // heads of a token side by side in a workgroup: 1 or 2
   int heads, heads_per_split, n_splits;
   FastDiv div_n, div_half;
   float* partial;  // backward: [grid_tiles n_splits][2][D] sums of the gains' gradients

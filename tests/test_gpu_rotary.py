@@ -405,3 +405,26 @@ def test_no_second_derivative():
     (g,) = torch.autograd.grad(y.square().sum(), q, create_graph=True)
     with pytest.raises(RuntimeError):
         g.square().sum().backward()
+
+
+@pytest.mark.parametrize("dtype,D,rd,inter,H,Hkv,n", [
+    (BF16, 128, 128, False, 31, 9, 17001), (F16, 40, 32, True, 41, 3, 41000),
+    (F32, 256, 64, False, 9, 4, 11003), (BF16, 72, 72, False, 1, 1, 499999)])
+def test_long_rows_of_one_projection(dtype, D, rd, inter, H, Hkv, n):
+    """More than the last-level cache holds, a token's heads side by side: the
+    same bits as head by head, for the forward and an append."""
+    gen = torch.Generator(device=DEV).manual_seed(12)
+    x = torch.randn(1, n, H + 2 * Hkv, D, generator=gen, device=DEV).to(dtype)
+    q, k, v = (t.transpose(1, 2) for t in x.split((H, Hkv, Hkv), 2))
+    layer = QKNormRope(D, rd, base=5e5, interleaved=inter).to(DEV).to(dtype)
+    pos = torch.arange(7, n + 7, device=DEV)
+    with torch.no_grad():
+        layer.q_weight.uniform_(0.5, 1.5)
+        for a, b in zip(layer(q, k, pos), layer(q.contiguous(), k.contiguous(), pos)):
+            assert torch.equal(a, b)
+        caches = [[torch.zeros(1, Hkv, n + 9, D, dtype=dtype, device=DEV) for _ in "kv"]
+                  for _ in range(2)]
+        a = layer.append(q, k, v, *caches[0], pos)
+        b = layer.append(q.contiguous(), k.contiguous(), v.contiguous(), *caches[1], pos)
+    assert torch.equal(a, b)
+    assert all(torch.equal(x, y) for x, y in zip(*caches))
