@@ -642,3 +642,46 @@ def test_many_sequences_and_heads(B, H, Hkv, Lq, Lk):
     assert torch.equal(caches[0], want_k) and torch.equal(caches[1], want_v)
     want, _ = sink_window_attention_fwd(yq, want_k, want_v, W, S, D ** -0.5, pos.to(DEV))
     assert torch.equal(got, want.view(B, Lq, H * D))
+
+
+def test_two_threads_on_two_streams():
+    """Steps, prefills and backward passes of two threads at once, each on its
+    own stream, are what each gives alone."""
+    import threading
+    D, H, Hkv = 64, 4, 2
+    rotary = QKNormRope(D).to(DEV).to(BF16)
+    layer = SinkWindowAttention(H, D, 90, 4, Hkv, rotary=rotary)
+
+    def work(seed):
+        gen = torch.Generator(device=DEV).manual_seed(seed)
+        new = lambda *s: torch.randn(*s, generator=gen, device=DEV).to(BF16)
+        kc, vc = new(2, Hkv, 700, D), new(2, Hkv, 700, D)
+        out = []
+        for i in range(6):
+            n = (1, 5, 140)[i % 3]
+            q, k, v = new(2, H, n, D), new(2, Hkv, n, D), new(2, Hkv, n, D)
+            with torch.no_grad():
+                at = torch.arange(n, device=DEV) + 100 * i
+                out.append(layer(q, k, v, cache_position=at, kv_cache=(kc, vc))[0])
+            q, k, v = (t.requires_grad_() for t in (q, k, v))
+            o = layer(q, k, v)[0]
+            out += [o.detach(), *torch.autograd.grad(o, (q, k, v), torch.ones_like(o))]
+        return out
+
+    want = [work(s) for s in (1, 2)]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def run(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got[i] = work(i + 1)
+        stream.synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(got, want):
+        assert a is not None and all(torch.equal(x, y) for x, y in zip(a, b))
