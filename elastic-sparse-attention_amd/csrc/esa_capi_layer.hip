@@ -271,12 +271,14 @@ int sink_qpad(int q_len) { return (q_len + 3) / 4 * 4; }
 // blocks counted on 256 slots 76 us, on 512 100); a chunk costs what its stages
 // do and about `part` stages more for its float32 part (written, read and
 // joined; one where float32 products make a stage itself as long).  Counted so, with the blocks alike (a window):
-//   a sinks' block is cut into pieces of a window block's size;
+//   a sinks' block is cut into pieces of a window block's size, or of its chunks';
 //   of all blocks the whole rounds stay whole, and those that would run as an
-//   unfilled last round (or all of a grid too small for one) are cut so that
-//   they fill it together (8192 rows, 8 kv heads of 4 query heads, window 1024
-//   and 4 sinks, head_dim 128: 568 blocks on 512 slots, two rounds of 72 stages
-//   against one and a fifth: 480 us and 365, before the kernel itself was faster);
+//   unfilled last round are cut so that they fill it together (8192 rows, 8 kv
+//   heads of 4 query heads, window 1024 and 4 sinks, head_dim 128: 568 blocks on
+//   512 slots, two rounds of 72 stages against one and a fifth: 480 us and 365,
+//   before the kernel itself was faster);
+//   or all are cut, where that ends sooner (4096 rows, 32 heads on one kv head,
+//   window 512: 32 blocks of 320 stages, backward 692 us whole, 205 cut);
 // where the first blocks see many more rows than the last (a window near the
 // sequence's length) all are cut alike, to at most 2/3 of a slot's share.
 void sink_bwd_plan(SinkArgs& g) {
@@ -295,17 +297,17 @@ void sink_bwd_plan(SinkArgs& g) {
   int64_t cut = 1, n_last = 0, cut_last = 1;
   if (!alike && n_reg > 0) {
     const double share = (double)kv * n_reg * one * mean / (double)slots;
-    cut = (int64_t)std::max(1.0, std::min(8.0, std::ceil(1.5 * one / share)));
+    cut = (int64_t)std::max(1.0, std::min(64.0, std::ceil(1.5 * one / share)));
     cut = std::max<int64_t>(1, std::min<int64_t>(cut, 4 * slots / (kv * n_reg)));
   }
   // the sinks' pieces as long as the others' chunks, within 256 MiB of parts
-  int64_t sink_cut = 1;
-  if (n_sink > 0) {
-    const int64_t piece = std::max<int64_t>(1, one / cut);
-    sink_cut = std::min<int64_t>(64, (stages(g.q_len) + piece - 1) / piece);
-    sink_cut = std::min(sink_cut, std::max<int64_t>(1, 2048 / (kv * n_sink)));
-  }
-  const int64_t pieces = kv * n_sink * sink_cut, total = pieces + kv * n_reg;
+  auto sinks_cut = [&](int64_t piece) {
+    if (n_sink == 0) return int64_t(1);
+    const int64_t c = (stages(g.q_len) + piece - 1) / std::max<int64_t>(1, piece);
+    return std::max<int64_t>(1, std::min<int64_t>({c, 128, 2048 / (kv * n_sink)}));
+  };
+  int64_t sink_cut = sinks_cut(std::max<int64_t>(1, one / cut));
+  const int64_t total = kv * n_sink * sink_cut + kv * n_reg;
   if (alike && n_reg > 0 && total % slots != 0 && total < 8 * slots) {
     // the time, in stages, of `whole` blocks and then `chunks` chunks of `size`,
     // each taken by the next free slot
@@ -317,15 +319,29 @@ void sink_bwd_plan(SinkArgs& g) {
     };
     int64_t best = time(total, 0, one);
     const int64_t over = std::min<int64_t>(n_reg, (total % slots + kv - 1) / kv);
-    for (const int64_t n : {over, n_reg})
-      for (int64_t c = 2; c <= 16 && c <= one && kv * n * c <= 4 * slots; ++c) {
-        const int64_t t = time(total - kv * n, kv * n * c, (one + c - 1) / c + part);
+    for (int64_t c = 2; c <= 16 && c <= one; ++c) {
+      const int64_t piece = (one + c - 1) / c;
+      // the blocks past the whole rounds alone, then all of them and the sinks'
+      if (kv * over * c <= 4 * slots) {
+        const int64_t t = time(total - kv * over, kv * over * c, piece + part);
         if (t < best) {
           best = t;
-          n_last = n;
+          n_last = over;
           cut_last = c;
         }
       }
+      if (kv * n_reg * c <= 4 * slots) {
+        const int64_t cs = sinks_cut(piece);
+        const int64_t size = std::max(piece, (stages(g.q_len) + cs - 1) / cs * (n_sink > 0));
+        const int64_t t = time(0, kv * (n_sink * cs + n_reg * c), size + part);
+        if (t < best) {
+          best = t;
+          n_last = n_reg;
+          cut_last = c;
+        }
+      }
+    }
+    if (n_last == n_reg) sink_cut = sinks_cut((one + cut_last - 1) / cut_last);
   }
   g.cls_n[0] = n_sink;
   g.cls_cut[0] = (int)sink_cut;

@@ -754,7 +754,21 @@ __global__ __launch_bounds__(256) void sink_join_kernel(SinkArgs A) {
     f32x16 x = f32x16{};
     const float* part = A.partial + (it.part * 4 + quarter) * (2 * ND * 16 * 64) +
                         w * (16 * 64) + lane;
-    for (int c = 0; c < n; ++c, part += 4 * 2 * ND * 16 * 64)
+    // (four parts on their way at a time, added in order)
+    constexpr int64_t STEP = 4 * 2 * ND * 16 * 64;
+    int c = 0;
+    for (; c + 4 <= n; c += 4, part += 4 * STEP) {
+      float y[4][16];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[u][e] = part[u * STEP + e * 64];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] += y[u][e];
+    }
+    for (; c < n; ++c, part += STEP)
 #pragma unroll
       for (int e = 0; e < 16; ++e) x[e] += part[e * 64];
     float sum = 0.f;

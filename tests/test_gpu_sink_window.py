@@ -685,3 +685,11 @@ def test_two_threads_on_two_streams():
         t.join()
     for a, b in zip(got, want):
         assert a is not None and all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("H,L,D,W,S,dtype", [
+    (16, 1500, 128, 200, 4, BF16), (12, 1111, 64, 300, 130, F16), (24, 700, 64, 700, 0, BF16),
+    (8, 900, 64, 120, 4, F32)])
+def test_many_heads_on_one_kv_head(H, L, D, W, S, dtype):
+    """Few key blocks with many rows each: all of them cut into chunks."""
+    run_case(1, H, 1, L, L, D, W, S, dtype, [0], None, True, 31)
