@@ -187,47 +187,74 @@ void sink_pattern(SinkArgs& g, const esa_window* w) {
   g.nqb = (g.q_len + 127) / 128;
 }
 
-// Keys that a call's rows walk, at most.
-int64_t sink_keys(const SinkArgs& g) {
-  return std::min<int64_t>(g.kv_len, (int64_t)g.window + g.sinks + g.q_len);
-}
-
+// Which forward kernel, and into how many key ranges side by side.
+//
 // Few rows against many keys take the decode kernel (row tiles of 16 over the
-// heads that share a kv head, the keys cut into ranges side by side), others
-// the forward's 128-row blocks, which walk their keys one after the other.
-// Both estimated: a block walks a key in 0.026 us (float32: 0.08, at head_dim
-// past 64 0.14), blocks past the chip's slots wait for a round; the decode
-// kernel does 27000 (tile, key) pairs a microsecond at head_dim 64, 13500 at
-// 128 (float32: 13000, 4900), after 8 us.  Measured, decode against blocks:
-// bf16, head_dim 128, 32 heads on 8, window 4096, one sequence, 1 / 16 / 64
-// rows 13 / 17 / 37 us against 94 / 96 / 99; 8 sequences, 4 / 16 / 32 rows 33 /
-// 96 / 153 against 107 / 107 / 108; 64 sequences, window 1024, 8 / 16 / 32 rows
-// 82 / 157 / 306 against 149 / 147 / 147; head_dim 64, 64 sequences, 8 / 16 rows
-// 46 / 84 against 58 / 59; float32, 16 sequences, 16 heads on 4 of 64, window
-// 2048, 16 / 32 / 64 rows 67 / 83 / 134 against 160 / 161 / 170; 8 sequences, 8
-// heads on 2 of 128, window 1024, 64 rows 57 against 162.
-bool sink_decodes(const SinkArgs& g) {
-  if ((int64_t)g.B * g.H * g.q_len >= kMaxGrid / 4) return false;
+// heads that share a kv head, the keys cut into ranges), others the forward's
+// 128-row blocks, which walk their keys one after the other; blocks that leave
+// CUs idle, or of which a few walk far more keys than the rest (a whole
+// sequence's last rows), are cut into ranges too.  All are estimated.
+//   decode: (tile, key) pairs a microsecond, after 8 us
+//   blocks: a CU with 1, 2, .. of them walks a key of all in `walk` us (16-bit
+//     128 dims: 158 us for two of 4227 keys each, 2110 for 8192 blocks, three a
+//     CU; float32 gains nothing from a second), after 6 us; ranges add 10 and
+//     their float32 parts, written and read at 4 TB/s
+// Measured, decode against blocks (not cut): bf16, head_dim 128, 32 heads on 8,
+// window 4096, one sequence, 1 / 16 / 64 rows 13 / 17 / 37 us against 94 / 96 /
+// 99; 8 sequences, 4 / 16 / 32 rows 33 / 96 / 153 against 107 / 107 / 108; 64
+// sequences, window 1024, 8 / 16 / 32 rows 82 / 157 / 306 against 149 / 147 /
+// 147; head_dim 64, 64 sequences, 8 / 16 rows 46 / 84 against 58 / 59; float32,
+// 16 sequences, 16 heads on 4 of 64, window 2048, 16 / 32 / 64 rows 67 / 83 / 134
+// against 160 / 161 / 170; 8 sequences, 8 heads on 2 of 128, window 1024, 64 rows
+// 57 against 162.  Blocks whole and cut (ranges): 2048 rows over 32768 keys, 4
+// heads on one of 128 866 and 165 us (12); 1024 rows, 32 heads on 8 875 and 579
+// (3); 512 rows, window 4096 118 and 68 (4); a sequence of 4096, 8 heads on 2 120
+// and 79 (4); 2048 rows, 32 heads, window 4096 176 and 202 (2).
+//
+// Key ranges of the decode kernel: as many as make 512 workgroups (two a CU:
+// with 1024 a 64-sequence step took 191 us against 184, four long sequences 102
+// against 94), each of at least 128 keys, 32 a wave (one sequence over 1028
+// keys: 9.9 us with 128, 11.3 with 256).
+void sink_fwd_plan(SinkArgs& g) {
   const bool f32 = g.elem == ESA_F32, narrow = g.d_real <= 64;
-  const double keys = (double)sink_keys(g);
-  const double tiles = (double)g.B * g.Hkv * (((int64_t)g.groups * g.q_len + 15) / 16);
+  const int64_t rows = (int64_t)g.B * g.H * g.q_len;
+  const int64_t tiles = (int64_t)g.B * g.Hkv * (((int64_t)g.groups * g.q_len + 15) / 16);
   const int64_t blocks = (int64_t)g.B * g.H * g.nqb;
-  const int64_t slots = f32 ? (narrow ? 512 : 256) : narrow ? 768 : 512;
+  // the keys that a tile's, a block's rows walk, at most; a block on average
+  // (whole sequences start with few)
+  const int64_t seen = (int64_t)g.window + g.sinks;
+  const int64_t tile_keys = std::min<int64_t>(g.kv_len, seen + std::min(g.q_len, 16));
+  const double keys = (double)std::min<int64_t>(g.kv_len, seen + std::min(g.q_len, 128));
+  const double mean = g.pos ? keys
+                            : std::min(keys, 128.0 + g.sinks +
+                                                 g.window * (1.0 - 0.5 * g.window / g.kv_len));
   const double rate = f32 ? (narrow ? 13000.0 : 4900.0) : narrow ? 27000.0 : 13500.0;
-  const double walk = f32 ? (narrow ? 0.08 : 0.14) : 0.026;
-  return tiles * keys / rate + 8.0 < keys * walk * (double)((blocks + slots - 1) / slots) ||
-         (int64_t)g.groups * g.q_len <= 16;
-}
-
-// Key ranges a row tile: as many as make 512 workgroups (two a CU: with 1024
-// a 64-sequence step took 191 us against 184, four long sequences 102 against
-// 94), each of at least 128 keys, 32 a wave (one sequence over 1028 keys: 9.9
-// us with 128, 11.3 with 256).
-void sink_splits(SinkArgs& g) {
-  g.row_tiles = (g.groups * g.q_len + 15) / 16;
-  const int64_t keys = sink_keys(g);
-  const int64_t units = (int64_t)g.B * g.Hkv * g.row_tiles;
-  g.splits = (int)std::min<int64_t>((keys + 127) / 128, std::max<int64_t>(1, 512 / units));
+  static const double walks[3][4] = {{0.0265, 0.0374, 0.048, 0}, {0.0209, 0.0286, 0.0376, 0.049},
+                                     {0.08, 0, 0, 0}};
+  const double* walk = walks[f32 ? 2 : narrow ? 1 : 0];
+  const int64_t fit = f32 ? 1 : narrow ? 4 : 3;  // blocks of a CU at a time
+  const double scale = f32 && !narrow ? 1.8 : 1.0;
+  auto blocks_time = [&](int64_t c) {
+    const int64_t x = (blocks * c + 255) / 256;
+    const double all = (double)(x / fit) * walk[fit - 1] + (x % fit ? walk[x % fit - 1] : 0.0);
+    const double parts = c > 1 ? 10.0 + (double)rows * c * (narrow ? 64 : 128) * 8 / 4.0e6 : 0.0;
+    return 6.0 + scale / (double)c * std::max(keys * walk[std::min(x, fit) - 1], mean * all) + parts;
+  };
+  const bool few = rows < kMaxGrid / 4;  // (a row's index fits 32 bits, its join a grid)
+  g.splits = 1;
+  double best = blocks_time(1);
+  for (int64_t c = 2; few && c <= 64 && keys / c >= 256 && blocks * c <= 2048; ++c) {
+    const double t = blocks_time(c);
+    if (t < best) {
+      best = t;
+      g.splits = (int)c;
+    }
+  }
+  g.decode = few && (tiles * (double)tile_keys / rate + 8.0 < best ||
+                     (int64_t)g.groups * g.q_len <= 16);
+  if (g.decode)
+    g.splits = (int)std::min<int64_t>((tile_keys + 127) / 128, std::max<int64_t>(1, 512 / tiles));
+  if (few) g.row_tiles = (g.groups * g.q_len + 15) / 16;
 }
 
 SinkArgs sink_fwd_args(const esa_fwd_args* a, const esa_window* w) {
@@ -245,13 +272,13 @@ SinkArgs sink_fwd_args(const esa_fwd_args* a, const esa_window* w) {
   g.scale_log2 = (float)((double)a->sm_scale * 1.4426950408889634);
   g.ores = w->o_residual;
   sink_pattern(g, w);
-  if (sink_decodes(g)) sink_splits(g);
+  sink_fwd_plan(g);
   return g;
 }
 
-// bytes of the decode kernel's parts: O [.., 16][D], then (m, l, n) [.., 16]
+// bytes of the key ranges' parts: O [.., 16][D], then (m, l, n) [.., 16]
 size_t sink_fwd_workspace(const SinkArgs& g) {
-  if (!sink_decodes(g) || g.splits <= 1) return 0;
+  if (g.splits <= 1) return 0;
   const size_t rows = (size_t)g.B * g.Hkv * g.row_tiles * g.splits * 16;
   return rows * ((g.d_real <= 64 ? 64 : 128) + 3) * sizeof(float);
 }
@@ -456,8 +483,8 @@ esa_status esa_sink_window_fwd(const esa_fwd_args* a, const esa_window* w, void*
     g.part_ml = g.partial + (size_t)g.B * g.Hkv * g.row_tiles * g.splits * 16 *
                                 (g.d_real <= 64 ? 64 : 128);
   }
-  const hipError_t e = sink_decodes(g) ? launch_sink_decode(g, (hipStream_t)stream)
-                                       : launch_sink_fwd(g, (hipStream_t)stream);
+  const hipError_t e = g.decode ? launch_sink_decode(g, (hipStream_t)stream)
+                                : launch_sink_fwd(g, (hipStream_t)stream);
   return e == hipSuccess ? ESA_OK : ESA_ERR_HIP;
 }
 

@@ -40,10 +40,15 @@ struct SinkArgs {
   int nkb;
   int cls_n[3], cls_cut[3];
   float* partial;             // partial sums of the blocks with more than one chunk
-  // decode
-  int splits;                 // key ranges a (sequence, kv head, row tile)
-  int row_tiles;              // 16-row tiles of its groups * q_len rows
-  float* part_ml;             // [.., splits, 16] running max and sum
+  // Key ranges side by side (decode: of a (sequence, kv head, row tile); the
+  // forward: of a row block), whose parts a join kernel adds up: row i of a kv
+  // head's groups * q_len (row_of) leaves, for range s, O in partial[unit][D] and
+  // (m, l, n) in part_ml[unit][3], unit = ((bkv row_tiles + i / 16) splits + s) 16
+  // + i % 16
+  bool decode;                // the decode kernel's row tiles, or the forward's blocks
+  int splits;
+  int row_tiles;              // 16-row tiles of a kv head's rows
+  float* part_ml;
 };
 
 // Where a sequence's rows and keys start.  ok: the first position lies inside
@@ -98,14 +103,19 @@ __device__ __forceinline__ bool none_seen(int p0, int p1, int k0, int window, in
 // keys), the query heads that share it next to each other, so that an XCD
 // works on the same keys at a time.
 struct RowItem {
-  int b, kvh, h, qb;
+  int b, kvh, h, qb, split;
 };
 __device__ __forceinline__ RowItem row_item(const SinkArgs& A) {
   int item = blockIdx.x;
   if (A.xcd_runs) item = (item & 7) * ((int)gridDim.x >> 3) + (item >> 3);
+  RowItem it;
+  it.split = 0;
+  if (A.splits > 1) {
+    it.split = item % A.splits;
+    item /= A.splits;
+  }
   const int per = A.nqb * A.groups;
   const int bkv = item / per, rem = item - bkv * per;
-  RowItem it;
   it.qb = A.nqb - 1 - rem / A.groups;
   it.b = bkv / A.Hkv;
   it.kvh = bkv - it.b * A.Hkv;
@@ -605,5 +615,6 @@ __device__ void fix_row(const SinkArgs& A, int b, int h, int kvh, int row, int p
 hipError_t launch_sink_fwd(const SinkArgs& a, hipStream_t stream);
 hipError_t launch_sink_bwd(const SinkArgs& a, hipStream_t stream);
 hipError_t launch_sink_decode(const SinkArgs& a, hipStream_t stream);
+hipError_t launch_sink_rows_join(const SinkArgs& a, hipStream_t stream);
 
 }  // namespace esa

@@ -317,7 +317,7 @@ __global__ __launch_bounds__(256, 2) void sink_decode_kernel(SinkArgs A) {
 // The key ranges of one row, joined in order: GR groups of lanes take every
 // GR-th range, each lane 4 dims, then the groups' sums in LDS.
 template <int D, Elem E>
-__global__ __launch_bounds__(512) void sink_decode_join_kernel(SinkArgs A) {
+__global__ __launch_bounds__(512) void sink_ranges_join_kernel(SinkArgs A) {
   using EL = typename ElemT<E>::T;
   constexpr int LPR = D / 4, GR = 512 / LPR;
   __shared__ __attribute__((aligned(16))) float ob[GR][D];
@@ -381,13 +381,70 @@ __global__ __launch_bounds__(512) void sink_decode_join_kernel(SinkArgs A) {
   }
 }
 
+// The same for the forward's blocks, many rows of few ranges: D / 4 lanes a row
+// go through its ranges in turn (65536 rows of two ranges at head_dim 128: 26 us,
+// with a workgroup a row 185).
+template <int D, Elem E>
+__global__ __launch_bounds__(256) void sink_rows_join_kernel(SinkArgs A) {
+  constexpr int LPR = D / 4, RPW = 64 / LPR;  // rows a wave
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n_rows = A.groups * A.q_len, n = A.B * A.Hkv * n_rows;
+  const int id0 = (blockIdx.x * 4 + wave) * RPW;
+  const bool in = id0 + lane / LPR < n;
+  const int id = min(id0 + lane / LPR, n - 1);
+  const int bkv = id / n_rows, ir = id - bkv * n_rows;
+  const int b = bkv / A.Hkv, kvh = bkv - b * A.Hkv;
+  const DecodeRow row = decode_row(A, kvh, ir);
+  const SeqInfo si = seq_info(A, b);
+  const int p = si.base + row.s, dim = 4 * (lane % LPR);
+  const int64_t u0 = (((int64_t)bkv * A.row_tiles + (ir >> 4)) * A.splits) * 16 + (ir & 15);
+  float mt = -INFINITY;
+  for (int s = 0; s < A.splits; ++s) mt = fmaxf(mt, A.part_ml[(u0 + 16 * s) * 3]);
+  const float mu = mt == -INFINITY ? 0.f : mt;
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
+  float lt = 0.f, nt = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < A.splits; ++s) {
+    const float* ml = A.part_ml + (u0 + 16 * s) * 3;
+    const float w = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - mu);
+    if (w != 0.f || ml[1] != ml[1]) {
+      lt += w * ml[1];
+      nt += w * ml[2];
+    }
+    y += w * *(const f32x4*)(A.partial + (u0 + 16 * s) * D + dim);
+  }
+  const bool valid = in && row_valid(A, si, b, row.s);
+  const float inv = !valid ? __builtin_nanf("") : p < si.first ? 0.f : 1.f / nt;
+  const int64_t orow = (int64_t)b * A.osb + (int64_t)row.h * A.osh + (int64_t)row.s * A.oss;
+  bool finite = __builtin_isfinite(lt);
+  if (dim < A.d_real) {
+    finite &= __builtin_isfinite((y[0] + y[1]) + (y[2] + y[3]));
+    if (in) store_out4<D, E>(A, orow, dim, y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+  }
+  if (in && A.lse && dim == 0)
+    A.lse[(int64_t)b * A.lsb + (int64_t)row.h * A.lsh + row.s] =
+        valid ? decode_lse(mt, lt, p < si.first) : __builtin_nanf("");
+  // rows that met a non-finite value, again from their own keys
+  const uint64_t bad = __builtin_amdgcn_ballot_w64(valid && !finite);
+  if (bad) __builtin_amdgcn_s_waitcnt(0);
+#pragma unroll 1
+  for (int q = 0; q < RPW; ++q) {
+    if ((bad >> (LPR * q) & ((uint64_t(1) << LPR) - 1)) == 0) continue;
+    const int fid = id0 + q, fkv = fid / n_rows, fb = fkv / A.Hkv, fh = fkv - fb * A.Hkv;
+    const DecodeRow fr = decode_row(A, fh, fid - fkv * n_rows);
+    const SeqInfo fi = seq_info(A, fb);
+    fix_row<E>(A, fb, fr.h, fh, fr.s, fi.base + fr.s, fi.first,
+               min(fi.first + A.sinks, A.kv_len), lane);
+  }
+}
+
 template <int D, Elem E>
 hipError_t launch_decode(const SinkArgs& a, hipStream_t stream) {
   const int64_t grid = (int64_t)a.B * a.Hkv * a.row_tiles * a.splits;
   sink_decode_kernel<D, E><<<(unsigned)grid, 256, 0, stream>>>(a);
-  hipError_t e = hipGetLastError();
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
-  sink_decode_join_kernel<D, E>
+  sink_ranges_join_kernel<D, E>
       <<<(unsigned)((int64_t)a.B * a.H * a.q_len), 512, 0, stream>>>(a);
   return hipGetLastError();
 }
@@ -397,7 +454,26 @@ hipError_t launch_elem(const SinkArgs& a, hipStream_t stream) {
   return a.d_real <= 64 ? launch_decode<64, E>(a, stream) : launch_decode<128, E>(a, stream);
 }
 
+template <int D, Elem E>
+hipError_t launch_rows_join(const SinkArgs& a, hipStream_t stream) {
+  constexpr int ROWS = 256 / (D / 4);
+  const int64_t rows = (int64_t)a.B * a.H * a.q_len;
+  sink_rows_join_kernel<D, E><<<(unsigned)((rows + ROWS - 1) / ROWS), 256, 0, stream>>>(a);
+  return hipGetLastError();
+}
+
+template <Elem E>
+hipError_t rows_join_elem(const SinkArgs& a, hipStream_t stream) {
+  return a.d_real <= 64 ? launch_rows_join<64, E>(a, stream) : launch_rows_join<128, E>(a, stream);
+}
+
 }  // namespace
+
+hipError_t launch_sink_rows_join(const SinkArgs& a, hipStream_t stream) {
+  if (a.elem == (int)Elem::f32) return rows_join_elem<Elem::f32>(a, stream);
+  if (a.elem == (int)Elem::bf16) return rows_join_elem<Elem::bf16>(a, stream);
+  return rows_join_elem<Elem::f16>(a, stream);
+}
 
 hipError_t launch_sink_decode(const SinkArgs& a, hipStream_t stream) {
   (void)hipGetLastError();

@@ -9,7 +9,9 @@
 // come in stages of 32 keys copied HBM -> LDS without registers, up to two
 // stages ahead.  A 32 x 32 block costs two products, S^T = K Q^T and
 // O^T += V^T P^T, with P straight from the accumulators; a stage of which a
-// wave sees nothing is skipped, one that it sees whole takes no mask.
+// wave sees nothing is skipped, one that it sees whole takes no mask.  Where a
+// grid leaves CUs idle a block's stages are cut into ranges, a workgroup each,
+// that leave (O, m, l) for a join.
 //
 // Bound: the vector instructions of a block (about 92 beside its 16 matrix
 // instructions at head_dim 128; a SIMD's vector and matrix pipes overlap in
@@ -63,8 +65,12 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
   const bool row_in = r < A.q_len;
   const int p = si.base + r;
   const int pb = keys.pb, pw0 = si.base + r0 + wave * 32, pw1 = min(pw0 + 31, pb);
-  const int n_all = keys.n_all;
-  const WaveStages ws = wave_stages(keys, pw0, pw1, W, sink_end);
+  // this workgroup's range of the stages, from i0 (all of them, unless the grid
+  // is small and they are cut)
+  const int i0 = (int)((int64_t)keys.n_all * it.split / A.splits);
+  const int n_all = (int)((int64_t)keys.n_all * (it.split + 1) / A.splits);
+  WaveStages ws = wave_stages(keys, pw0, pw1, W, sink_end);
+  ws.last = min(ws.last, n_all - 1);
 
   T t;
   t.init(lane);
@@ -221,21 +227,21 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
       vs.issue(keys.key0(i), vd, wave);
     }
   };
-  issue(0, k0_, v0_);
-  issue(1, k1_, v1_);
-  if (n_all > 0) {
-    if (n_all > 1)
+  issue(i0, k0_, v0_);
+  issue(i0 + 1, k1_, v1_);
+  if (n_all > i0) {
+    if (n_all > i0 + 1)
       stage_wait<3 * Stage::LOADS>();
     else
       stage_wait<0>();
-    if (ws.sees(0)) {
+    if (ws.sees(i0)) {
       t.row_product(s, k0_, 0, qf);
       top = row_top(s);
-      hide(s, top, 0);
+      hide(s, top, i0);
       used = true;
     }
   }
-  for (int i = 0; i < n_all; i += 3) {
+  for (int i = i0; i < n_all; i += 3) {
     ready(i);
     issue(i + 2, k2_, v2_);
     step(v0_, k1_, i);
@@ -253,6 +259,27 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
   const bool met = row_in && !(sum_finite(oacc) && __builtin_isfinite(l_run));
   const float l_tot = l_run + __shfl_xor(l_run, 32, 64);
   const float n_tot = n_run + __shfl_xor(n_run, 32, 64);
+  if (A.splits > 1) {  // a part
+    const int i = r * A.groups + h - kvh * A.groups;
+    const int64_t unit = (((int64_t)(b * A.Hkv + kvh) * A.row_tiles + (i >> 4)) * A.splits +
+                          it.split) * 16 + (i & 15);
+    if (row_in) {
+      float* row = A.partial + unit * D + 4 * hf;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *(f32x4*)(row + 32 * d + 8 * q) = f32x4{oacc[d][4 * q], oacc[d][4 * q + 1],
+                                                  oacc[d][4 * q + 2], oacc[d][4 * q + 3]};
+      if (hf == 0) {
+        float* ml = A.part_ml + unit * 3;
+        ml[0] = m_run;
+        ml[1] = l_tot;
+        ml[2] = n_tot;
+      }
+    }
+    return;
+  }
   // a row that sees no key (before the sequence's first one): 0 and -inf; one
   // without a place in the cache: NaN
   const bool valid = row_in && row_valid(A, si, b, r);
@@ -280,7 +307,7 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
 
 template <Elem E>
 void launch_elem(const SinkArgs& a, hipStream_t stream) {
-  const int64_t grid = (int64_t)a.B * a.H * a.nqb;
+  const int64_t grid = (int64_t)a.B * a.H * a.nqb * a.splits;
   SinkArgs g = a;
   g.xcd_runs = sink_xcd_runs(a, grid);
   if (a.d_real <= 64)
@@ -299,7 +326,8 @@ hipError_t launch_sink_fwd(const SinkArgs& a, hipStream_t stream) {
     launch_elem<Elem::bf16>(a, stream);
   else
     launch_elem<Elem::f16>(a, stream);
-  return hipGetLastError();
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess || a.splits == 1 ? e : launch_sink_rows_join(a, stream);
 }
 
 }  // namespace esa

@@ -693,3 +693,53 @@ def test_two_threads_on_two_streams():
 def test_many_heads_on_one_kv_head(H, L, D, W, S, dtype):
     """Few key blocks with many rows each: all of them cut into chunks."""
     run_case(1, H, 1, L, L, D, W, S, dtype, [0], None, True, 31)
+
+
+@pytest.mark.parametrize("dtype,D,Lq,W", [(BF16, 128, 300, 5000), (F16, 64, 513, 3000),
+                                          (BF16, 72, 300, 5000), (F32, 64, 600, 5000)])
+def test_blocks_cut_into_key_ranges(dtype, D, Lq, W):
+    """A chunk of few heads over a long cache: row blocks whose keys are walked
+    in ranges side by side, with left padding, Inf and NaN where no row looks, one
+    visible Inf, rows without a place, and from a graph."""
+    H, Lk, S, first = 4, 5000, 3, 700
+    q, k, v, gen = make(1, H, 1, Lq, Lk, D, dtype, False, 41)
+    pos = Lk - 90 - Lq + torch.arange(Lq)[None]
+    f = torch.tensor([first])
+    seen = window_mask(pos, f, Lk, W, S)
+    scale = D ** -0.5
+    ref, tol = bounds(q, k, v, seen, scale, dtype)
+    hidden = ~seen.any(1)
+    k, v = plant(k, hidden, gen), plant(v, hidden, gen)
+    qd, kd, vd = q.to(DEV), k.to(DEV), v.to(DEV)
+    args = (W, S, scale, pos.to(DEV), f.to(DEV))
+    o, lse, res = sink_window_attention_fwd(qd, kd, vd, *args, return_residual=True)
+    close(o.transpose(1, 2), ref[0], tol[0], "o")
+    close(lse, ref[1], tol[1], "lse")
+    if res is not None:
+        u = torch.finfo(dtype).eps / 2
+        both = (o.double() + res.double()).transpose(1, 2).cpu()
+        assert bool(((both - ref[0]).abs() <= tol[0] + u * u * ref[0].abs() + 2.0 ** -24).all())
+    assert torch.equal(sink_window_attention_fwd(qd, kd, vd, *args, return_lse=False)[0], o)
+    vi = vd.clone()
+    vi[0, 0, Lk - 90 - Lq, 5] = math.inf  # the first row's own key: every row's, or the window's
+    oi, li = sink_window_attention_fwd(qd, kd, vi, *args)
+    sees = seen[0, :, Lk - 90 - Lq].to(DEV)
+    assert torch.isposinf(oi[0, sees, :, 5]).all() and torch.isfinite(oi[0, :, :, 6:]).all()
+    assert torch.equal(li, lse) or torch.allclose(li, lse, rtol=1e-5, atol=1e-5)
+    late = pos.to(DEV) + 120             # the last rows past the cache's end
+    ol, ll = sink_window_attention_fwd(qd, torch.nan_to_num(kd), torch.nan_to_num(vd), W, S, scale,
+                                       late, f.to(DEV))
+    out = (late[0] >= Lk)
+    assert out.any() and torch.isnan(ol[0, out]).all() and torch.isnan(ll[0, :, out]).all()
+    # (keys behind pos hold anything, what nan_to_num makes of Inf among it: q k
+    # overflows there, and the formula gives NaN; rows before them are finite)
+    assert torch.isfinite(ol[0, late[0] <= int(pos.max())]).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        og, lg, _ = sink_window_attention_fwd(qd, kd, vd, *args, return_residual=True)
+    for _ in range(3):
+        og.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(og, o) and torch.equal(lg, lse)
+        sink_window_attention_fwd(qd, kd, vi, *args)
