@@ -601,8 +601,9 @@ typedef struct esa_window {
   void* o_residual;
 } esa_window;
 
-/* Host only.  Workspace of esa_sink_window_fwd: 0 but for a few rows against
- * many keys, whose key ranges are computed side by side and joined. */
+/* Host only.  Workspace of esa_sink_window_fwd: 0 but where key ranges are
+ * computed side by side and joined (few rows, or few blocks of 128 rows, against
+ * many keys). */
 esa_status esa_sink_window_fwd_workspace_size(const esa_fwd_args* a, const esa_window* w,
                                               size_t* bytes);
 
