@@ -318,7 +318,6 @@ __global__ __launch_bounds__(256, 2) void sink_decode_kernel(SinkArgs A) {
 // GR-th range, each lane 4 dims, then the groups' sums in LDS.
 template <int D, Elem E>
 __global__ __launch_bounds__(512) void sink_ranges_join_kernel(SinkArgs A) {
-  using EL = typename ElemT<E>::T;
   constexpr int LPR = D / 4, GR = 512 / LPR;
   __shared__ __attribute__((aligned(16))) float ob[GR][D];
   __shared__ float wsum[GR][2];
