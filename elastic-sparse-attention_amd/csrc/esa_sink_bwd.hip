@@ -104,10 +104,10 @@ __device__ void fix_dq_row(const SinkArgs& A, int b, int h, int kvh, int row, in
     if (lane + 64 * c < A.d_real) T::store(dq + lane + 64 * c, acc[c]);
 }
 
-template <int D, Elem E>
+template <int D, int DR, Elem E>
 __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::DQ_WAVES)) void sink_dq_kernel(
     SinkArgs A) {
-  using T = SinkTile<D, E>;
+  using T = SinkTile<D, E, false, DR>;
   using Stage = SinkStage<D, E, 32, 256>;
   using LdsT = typename T::LdsT;
   constexpr int ND = T::ND, N = 32 * D;
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::DQ_WAVES)) void sink_dq_ker
     f32x16 sn = f32x16{}, dp = f32x16{};
     if constexpr (T::ES == 2) {
       // in written order, operands read AHEAD products ahead
-      constexpr int AHEAD = 4, NS = T::NS, PER = 8 / NS;  // PER: pairs of keys a product
+      constexpr int AHEAD = 4, NS = T::NS;
       typename T::V8 va[NS], ka[NS];
       u32x4 kc[NS];
       typename T::P pd;
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::DQ_WAVES)) void sink_dq_ker
       };
       auto grads = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
-        for (int q = k * PER; q < (k + 1) * PER; ++q) {
+        for (int q = 8 * k / NS; q < 8 * (k + 1) / NS; ++q) {  // pairs of keys (rows)
 #pragma unroll
           for (int e = 2 * q; e < 2 * q + 2; ++e) s[e] *= dp[e] - delta;
           pd.w[q] = T::M::pack2(s[2 * q], s[2 * q + 1]);
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::DQ_WAVES)) void sink_dq_ker
         dp = T::M::mfma32(va[k], gf.f[k], dp);
         read(k + AHEAD);
 #pragma unroll
-        for (int e = 2 * k * PER; e < 2 * (k + 1) * PER; ++e)
+        for (int e = 2 * (8 * k / NS); e < 2 * (8 * (k + 1) / NS); ++e)
           s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], scale, -lse2));
       }
       // (past the wave's last key: of whatever the buffer holds, and dropped)
@@ -369,17 +369,17 @@ __device__ __forceinline__ KeyItem key_item(const SinkArgs& A) {
 }
 
 // Stores 32 keys' dK^T and dV^T (one wave's accumulators; in: the lane's key is one)
-template <int D, Elem E>
+template <int D, int DR, Elem E>
 __device__ __forceinline__ void store_keys(const SinkArgs& A, int b, int kvh, int j, int hf,
-                                           const f32x16 (&dk)[SinkTile<D, E>::ND],
-                                           const f32x16 (&dv)[SinkTile<D, E>::ND], bool in) {
+                                           const f32x16 (&dk)[DR / 32],
+                                           const f32x16 (&dv)[DR / 32], bool in) {
   using T = SinkTile<D, E>;
   auto* kr = (typename ElemT<E>::T*)A.dk + (int64_t)b * A.dksb + (int64_t)kvh * A.dksh +
              (int64_t)j * A.dkss;
   auto* vr = (typename ElemT<E>::T*)A.dv + (int64_t)b * A.dvsb + (int64_t)kvh * A.dvsh +
              (int64_t)j * A.dvss;
 #pragma unroll
-  for (int d = 0; d < T::ND; ++d) {
+  for (int d = 0; d < DR / 32; ++d) {
     T::store32(kr, 32 * d, dk[d], A.sm_scale, hf, A.d_real, in);
     T::store32(vr, 32 * d, dv[d], 1.f, hf, A.d_real, in);
   }
@@ -449,11 +449,11 @@ __device__ __forceinline__ void fix_keys(const SinkArgs& A, const SeqInfo& si, i
   }
 }
 
-template <int D, Elem E>
+template <int D, int DR, Elem E>
 __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::KV_WAVES)) void sink_dkdv_kernel(
     SinkArgs A) {
   using C = SinkBwdCfg<D, E>;
-  using T = SinkTile<D, E, (D >= 128)>;
+  using T = SinkTile<D, E, (D >= 128), DR>;
   using Stage = SinkStage<D, E, C::ROWS, 256>;
   using LdsT = typename T::LdsT;
   constexpr int ND = T::ND;
@@ -579,12 +579,18 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::KV_WAVES)) void sink_dkdv_k
       // The four products in written order, each beside the vector work of the
       // one before it (S: none; dP: P's exponentials; dV: dS; dK: dS's rest),
       // operands read AHEAD products ahead.
-      constexpr int AHEAD = 3, NS = T::NS, PER = 8 / NS;  // products of each; pairs of rows a product
+      constexpr int AHEAD = 3, NS = T::NS;  // products of each
       typename T::V8 qa[NS], ga[NS], va[NS];
       int base;  // of the reads' addresses
       u32x4 gc[NS], qc[NS];
       typename T::P pp, pd;
       f32x4 l2[4], dl[4];
+      // beside product k: the lse or delta of the four rows after its own pairs'
+      auto ahead_stat = [&](f32x4 (&to)[4], int at, int k) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q4 = 1; q4 < 4; ++q4)
+          if (2 * q4 - 2 >= 8 * k / NS && 2 * q4 - 2 < 8 * (k + 1) / NS) to[q4] = row_stat(at, q4);
+      };
       auto read = [&](int i) __attribute__((always_inline)) {  // operands in their order
         const int k = i % NS;
         if (i < 2 * NS) {
@@ -605,7 +611,7 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::KV_WAVES)) void sink_dkdv_k
       };
       auto exps = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
-        for (int q = k * PER; q < (k + 1) * PER; ++q) {
+        for (int q = 8 * k / NS; q < 8 * (k + 1) / NS; ++q) {  // pairs of keys (rows)
 #pragma unroll
           for (int e = 2 * q; e < 2 * q + 2; ++e)
             s[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], scale, -l2[e / 4][e % 4]));
@@ -614,7 +620,7 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::KV_WAVES)) void sink_dkdv_k
       };
       auto grads = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
-        for (int q = k * PER; q < (k + 1) * PER; ++q) {
+        for (int q = 8 * k / NS; q < 8 * (k + 1) / NS; ++q) {  // pairs of keys (rows)
 #pragma unroll
           for (int e = 2 * q; e < 2 * q + 2; ++e) s[e] *= dp[e] - dl[e / 4][e % 4];
           pd.w[q] = T::M::pack2(s[2 * q], s[2 * q + 1]);
@@ -636,10 +642,7 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::KV_WAVES)) void sink_dkdv_k
         __builtin_amdgcn_sched_barrier(0);
         dp = T::M::mfma32(ga[k], C::V_LDS ? va[k] : vf.f[k], dp);
         read(NS + k + AHEAD);
-        if (PER == 2 || k % 2 == 0) {
-          const int q4 = (k * PER) / 2 + 1;
-          if (q4 < 4) l2[q4] = row_stat(0, q4);
-        }
+        ahead_stat(l2, 0, k);
         if (k > 0) exps(k - 1);
       }
       dl[0] = row_stat(64, 0);
@@ -648,10 +651,7 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::KV_WAVES)) void sink_dkdv_k
         __builtin_amdgcn_sched_barrier(0);
         T::col_step(dv[k % ND], gc[k], pp, k / ND);
         read(2 * NS + k + AHEAD);
-        if (PER == 2 || k % 2 == 0) {
-          const int q4 = (k * PER) / 2 + 1;
-          if (q4 < 4) dl[q4] = row_stat(64, q4);
-        }
+        ahead_stat(dl, 64, k);
         if (k == 0) exps(NS - 1);
         if (k > 0) grads(k - 1);
       }
@@ -718,15 +718,15 @@ __global__ __launch_bounds__(256, (SinkBwdCfg<D, E>::KV_WAVES)) void sink_dkdv_k
     return;
   }
   const bool met = key_in && !(sum_finite(dk) && sum_finite(dv));
-  store_keys<D, E>(A, b, kvh, j, hf, dk, dv, key_in);
+  store_keys<D, DR, E>(A, b, kvh, j, hf, dk, dv, key_in);
   fix_keys<E>(A, si, b, kvh, jw0, sink_end, met, lane);
 }
 
 // The parts of one cut key block's 32 keys, summed in their order: each wave
 // takes the 32-dim pieces of dK and dV in turn.
-template <int D, Elem E>
+template <int D, int DR, Elem E>
 __global__ __launch_bounds__(256) void sink_join_kernel(SinkArgs A) {
-  using T = SinkTile<D, E>;
+  using T = SinkTile<D, E, false, DR>;
   constexpr int ND = T::ND;
   __shared__ uint32_t met[4][32];
   int n_cut = 0;
@@ -795,12 +795,12 @@ __global__ __launch_bounds__(256) void sink_join_kernel(SinkArgs A) {
   fix_keys<E>(A, si, it.b, it.kvh, jw0, sink_end, fix, lane);
 }
 
-template <int D, Elem E>
+template <int D, int DR, Elem E>
 hipError_t launch_bwd(const SinkArgs& a, hipStream_t stream) {
   SinkArgs g = a;
   const int64_t n_dq = (int64_t)a.B * a.H * a.nqb;
   g.xcd_runs = sink_xcd_runs(a, n_dq);
-  sink_dq_kernel<D, E><<<(unsigned)n_dq, 256, 0, stream>>>(g);
+  sink_dq_kernel<D, DR, E><<<(unsigned)n_dq, 256, 0, stream>>>(g);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   int64_t units = 0, n_cut = 0;
@@ -810,16 +810,17 @@ hipError_t launch_bwd(const SinkArgs& a, hipStream_t stream) {
   }
   const int64_t n_kv = (int64_t)a.B * a.Hkv * units;
   g.xcd_runs = sink_xcd_runs(a, n_kv);
-  sink_dkdv_kernel<D, E><<<(unsigned)n_kv, 256, 0, stream>>>(g);
+  sink_dkdv_kernel<D, DR, E><<<(unsigned)n_kv, 256, 0, stream>>>(g);
   e = hipGetLastError();
   if (e != hipSuccess || n_cut == 0) return e;
-  sink_join_kernel<D, E><<<(unsigned)(4 * a.B * a.Hkv * n_cut), 256, 0, stream>>>(g);
+  sink_join_kernel<D, DR, E><<<(unsigned)(4 * a.B * a.Hkv * n_cut), 256, 0, stream>>>(g);
   return hipGetLastError();
 }
 
 template <Elem E>
 hipError_t launch_elem(const SinkArgs& a, hipStream_t stream) {
-  return a.d_real <= 64 ? launch_bwd<64, E>(a, stream) : launch_bwd<128, E>(a, stream);
+  if (a.d_real <= 64) return launch_bwd<64, 64, E>(a, stream);
+  return a.d_real <= 96 ? launch_bwd<128, 96, E>(a, stream) : launch_bwd<128, 128, E>(a, stream);
 }
 
 }  // namespace

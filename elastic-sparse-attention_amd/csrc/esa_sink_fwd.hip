@@ -36,10 +36,10 @@ struct SinkFwdCfg {
       E == Elem::f32 ? (D >= 128 ? 1 : 2) : D >= 128 ? 3 : 4;
 };
 
-template <int D, Elem E>
+template <int D, int DR, Elem E>
 __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_fwd_kernel(
     SinkArgs A) {
-  using T = SinkTile<D, E, true>;
+  using T = SinkTile<D, E, true, DR>;
   using Stage = SinkStage<D, E, 32, 256>;
   using LdsT = typename T::LdsT;
   constexpr int ND = T::ND, N = 32 * D;
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
       // In written order, each operand read AHEAD products ahead: the first half
       // of the scores beside the first half of the exponentials, the second half
       // of both beside the first products with V, then V's rest.
-      constexpr int AHEAD = 3, NS = T::NS, H = NS / 2, PER = 8 / NS;
+      constexpr int AHEAD = 3, NS = T::NS, H = NS / 2;
       typename T::V8 ka[NS];
       u32x4 va[2 * ND];
       typename T::P pp;
@@ -169,7 +169,7 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
       };
       auto exps = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
-        for (int q = k * PER; q < (k + 1) * PER; ++q) {
+        for (int q = 8 * k / NS; q < 8 * (k + 1) / NS; ++q) {  // pairs of keys
           s[2 * q] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * q], scale, -m_use));
           s[2 * q + 1] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[2 * q + 1], scale, -m_use));
           l_run += s[2 * q] + s[2 * q + 1];
@@ -190,8 +190,8 @@ __global__ __launch_bounds__(256, (SinkFwdCfg<D, E>::WAVES_PER_SIMD)) void sink_
           T::col_step(oacc[k % ND], va[k], pp, k / ND);
           // O is normalised by the probabilities that its product used
 #pragma unroll
-          for (int w = 0; w < PER; ++w)
-            n_run = T::M::dot2(pp.w[4 * (k / ND) + PER * (k % ND) + w], n_run);
+          for (int w = 4 * (k % ND) / ND; w < 4 * (k % ND + 1) / ND; ++w)
+            n_run = T::M::dot2(pp.w[4 * (k / ND) + w], n_run);
           asm volatile("" : "+v"(n_run));
         }
         read(i + AHEAD);
@@ -311,9 +311,11 @@ void launch_elem(const SinkArgs& a, hipStream_t stream) {
   SinkArgs g = a;
   g.xcd_runs = sink_xcd_runs(a, grid);
   if (a.d_real <= 64)
-    sink_fwd_kernel<64, E><<<(unsigned)grid, 256, 0, stream>>>(g);
+    sink_fwd_kernel<64, 64, E><<<(unsigned)grid, 256, 0, stream>>>(g);
+  else if (a.d_real <= 96)
+    sink_fwd_kernel<128, 96, E><<<(unsigned)grid, 256, 0, stream>>>(g);
   else
-    sink_fwd_kernel<128, E><<<(unsigned)grid, 256, 0, stream>>>(g);
+    sink_fwd_kernel<128, 128, E><<<(unsigned)grid, 256, 0, stream>>>(g);
 }
 
 }  // namespace
